@@ -324,6 +324,107 @@ int ppo_xp_rnorm_step_finish_device(ppo_xp_rnorm *r, const float *rewards_dev, c
                                     float *out_dev, size_t n, void *stream);
 int ppo_xp_rnorm_state(ppo_xp_rnorm *r, float *mean, float *var, float *count, float *ret_out, size_t n);
 
+/* ---- policies whose actions are tokens -----------------------------------------------------------------------------
+ * What surrounds the buffer when an action is one of many tokens: the rules that shape the logits before an action is
+ * drawn, the neglogp that ppo_xp_add_device stores, the clipped objective over a gathered minibatch with its gradient,
+ * and observation rows kept in 8 or 4 bits.  The reference computes the first three inside its learner
+ * (ppo/src/model/learner.rs:112-244, ppo/src/model/util.rs:3-33) for a handful of actions.
+ *
+ * All calls below take device arrays of HIP device `device` and only ENQUEUE on `stream` (a hipStream_t of that device;
+ * NULL = its default stream): inputs must be ready on that stream, outputs are ready behind it.  The caller's current
+ * device is put back.  Nothing is allocated and nothing synchronises, so every call may be captured into a HIP graph.
+ * Rows may lie apart: every *_stride counts ELEMENTS from one row to the next (0 for one shared row where said so).
+ * rows == 0 or vocab == 0 does nothing.  Sums, maxima and statistics are held in 32 bits or more; results are rounded
+ * to the element type once. */
+
+enum { PPO_XP_F32 = 0, PPO_XP_BF16 = 1, PPO_XP_F16 = 2 };          /* element types                        */
+enum { PPO_XP_MASK_NONE = 0, PPO_XP_MASK_BITS = 1, PPO_XP_MASK_BYTES = 2 };
+
+/* How the logits of a row are shaped.  For token v of row r, with the row's history tokens at positions [begin, end):
+ *   x = logit
+ *   v occurs in [begin, end):             x = x > 0 ? x / repetition : x * repetition
+ *   v occurs c > 0 times in [gen, end):   x -= frequency * c + presence
+ *   x += bias[v];   x /= temperature;   mask forbids v: x = -inf (whatever the logit was, NaN included)
+ * Any pointer may be NULL: no such rule, or the default named below. */
+typedef struct ppo_xp_logit_rules {
+  const void *history;              /* token ids, history_bits wide; token k of history row h: history[h * row_stride + k * tok_stride],
+                                       so the buffer's time-major actions [T, N] serve with row_stride 1, tok_stride N.  Ids outside
+                                       0..vocab (padding, -1) are skipped                                                       */
+  int64_t hist_row_stride, hist_tok_stride;
+  int64_t hist_rows, hist_len;      /* history rows, and positions per row                                                      */
+  const int32_t *hist_row;          /* [rows] history row of each logits row (NULL: the row itself); one outside 0..hist_rows has none */
+  const int32_t *hist_begin;        /* [rows] first position (NULL: 0); positions are clamped to 0..hist_len                    */
+  const int32_t *gen_begin;         /* [rows] first position that counts for frequency / presence (NULL: begin)                 */
+  const int32_t *hist_end;          /* [rows] one past the last position (NULL: hist_len)                                       */
+  const float *repetition_rows, *presence_rows, *frequency_rows, *temperature_rows; /* [rows] per-row values (NULL: the scalars) */
+  const float *bias;                /* [rows, vocab] f32, added before the temperature                                          */
+  int64_t bias_stride;              /* 0: one bias row for all                                                                  */
+  const void *mask;                 /* BITS: u32 words, bit v % 32 of word v / 32 set = allowed; BYTES: one byte per token, non-zero = allowed */
+  int64_t mask_stride;              /* in words / bytes; 0: one mask row for all                                                */
+  int64_t mask_rows;                /* mask rows                                                                                */
+  const int32_t *mask_row;          /* [rows] mask row of each logits row (NULL: the row itself); one outside 0..mask_rows = unconstrained */
+  float repetition, presence, frequency, temperature;  /* scalars: 1, 0, 0, 1 change nothing; repetition and temperature > 0    */
+  int32_t history_bits;             /* 32 or 64                                                                                 */
+  int32_t mask_kind;                /* PPO_XP_MASK_*                                                                            */
+} ppo_xp_logit_rules;
+
+/* out[r, v] = the shaped logit, in the logits' type.  `out` may be `logits`. */
+int ppo_xp_shape_logits(int device, void *stream, int dtype, const void *logits, int64_t logits_stride, void *out,
+                        int64_t out_stride, size_t rows, size_t vocab, const ppo_xp_logit_rules *rules);
+/* Its gradient: out = d(loss)/d(logits) from grad = d(loss)/d(shaped).  Needs the logits only for the sign of tokens the history
+ * holds; forbidden tokens get 0.  Bias and penalties are constants.  `out` may be `grad`. */
+int ppo_xp_shape_logits_backward(int device, void *stream, int dtype, const void *grad, int64_t grad_stride,
+                                 const void *logits, int64_t logits_stride, void *out, int64_t out_stride, size_t rows,
+                                 size_t vocab, const ppo_xp_logit_rules *rules);
+
+/* neglogps[r] = -log softmax(logits[r])[actions[r]], entropies[r] = that distribution's entropy (util.rs:3-33).  A logit of -inf
+ * is a forbidden token.  Row by row: actions[r] == -1 is padding (both 0); any other action outside 0..vocab, or a row that holds
+ * NaN or +inf, gives NaN; a row that is -inf throughout gives neglogp +inf and entropy 0.  `workspace`: at least
+ * ppo_xp_policy_workspace() bytes, 16-byte aligned, not shared with a call that may run at the same time. */
+int ppo_xp_action_stats(int device, void *stream, int dtype, const void *logits, int64_t logits_stride,
+                        const int64_t *actions, float *neglogps, float *entropies, size_t rows, size_t vocab,
+                        void *workspace, size_t workspace_bytes);
+/* Bytes of workspace that ppo_xp_action_stats and ppo_xp_policy_loss need for these sizes. */
+size_t ppo_xp_policy_workspace(int dtype, size_t rows, size_t vocab);
+
+/* The streams of a gathered minibatch (ppo_batch_view) and the critic's new values, [rows] each. */
+typedef struct ppo_xp_policy_batch {
+  const int64_t *actions;           /* -1: padding, the row contributes nothing                    */
+  const float *old_values, *old_neglogps, *returns, *advantages;
+  const float *values;              /* the critic's values of these rows now                       */
+} ppo_xp_policy_batch;
+
+/* The clipped objective and its gradient (learner.rs:165-244), in one pass over the logits.  With nlp, H as above, v0 / v the old /
+ * new value and ratio = exp(old_neglogp - nlp):
+ *   pg = max(-A ratio, -A clamp(ratio, 1 - clip, 1 + clip)),   vl = max((v - ret)^2, (v0 + clamp(v - v0, -clip, clip) - ret)^2) / 2
+ *   loss = (sum pg + vf_coef sum vl - ent_coef sum H) / denom
+ * stats[6] = loss, policy, value, entropy, sum (nlp - old)^2 / 2, rows with |ratio - 1| > clip - each over denom.  dlogits
+ * (the logits' type; may be the logits themselves), dvalues [rows]; neglogps and entropies [rows] as ppo_xp_action_stats
+ * gives them.  denom > 0: the rows to divide by, padding not counted.  A row that is -inf throughout has gradient 0. */
+int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, int64_t logits_stride,
+                       const ppo_xp_policy_batch *batch, float clip, float ent_coef, float vf_coef, double denom,
+                       void *dlogits, int64_t dlogits_stride, float *dvalues, float *neglogps, float *entropies,
+                       float *stats, size_t rows, size_t vocab, void *workspace, size_t workspace_bytes);
+
+/* Rows in 8 or 4 bits with one f32 scale per `group` elements of a row (the last group may be shorter):
+ *   INT8 / INT4: scale = amax / 127 | 7 rounded to f32, code = x / scale rounded to nearest, ties to even
+ *   E4M3:        scale = the smallest power of two with amax / scale <= 448, code = x / scale rounded likewise (OCP e4m3fn)
+ * A group whose amax is below 2^-110 is stored as zeros; one that holds NaN or an infinity reads back as NaN throughout.
+ * INT4 packs element 2i into the low and 2i + 1 into the high half of byte i, two's complement, an odd row's last half 0. */
+enum { PPO_XP_Q_INT8 = 1, PPO_XP_Q_E4M3 = 2, PPO_XP_Q_INT4 = 3 };
+
+/* rows[n, width] -> store rows at .. at + n; codes_stride in bytes, scales_stride in floats.  at + n > store_rows =>
+ * PPO_XP_EINVAL (a ring that wraps takes two calls). */
+int ppo_xp_quantize_rows(int device, void *stream, int dtype, const void *rows, int64_t rows_stride, size_t n,
+                         size_t width, int format, size_t group, void *codes, int64_t codes_stride, float *scales,
+                         int64_t scales_stride, size_t store_rows, size_t at);
+/* out[j] = store row index[j], as dtype (code * scale, one rounding).  index: index_bits 32 (unsigned) or 64 wide, an entry
+ * outside 0..store_rows reads the last row (as in a pass, a bad index never faults); NULL: rows at .. at + n.  */
+int ppo_xp_dequantize_rows(int device, void *stream, int dtype, const void *codes, int64_t codes_stride,
+                           const float *scales, int64_t scales_stride, size_t store_rows, size_t width, int format,
+                           size_t group, const void *index, int index_bits, size_t at, size_t n, void *out,
+                           int64_t out_stride);
+
 /* ---- plumbing --------------------------------------------------------------------------- */
 
 void *ppo_xp_stream(const ppo_xp *h);            /* hipStream_t of the handle                */

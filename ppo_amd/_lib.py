@@ -58,6 +58,7 @@ class BatchHost(C.Structure):
 
 # name -> (restype, argtypes); every symbol include/ppo_xp.h declares.
 _vp, _sz, _i, _f, _u64 = C.c_void_p, C.c_size_t, C.c_int, C.c_float, C.c_uint64
+_i64, _d = C.c_int64, C.c_double
 SYMBOLS = {
     "ppo_xp_create": (_i, [C.POINTER(_vp), _i, _sz, _sz, _sz, _f, _f]),
     "ppo_xp_destroy": (None, [_vp]),
@@ -106,6 +107,13 @@ SYMBOLS = {
     "ppo_xp_rnorm_sums_device": (_vp, [_vp]),
     "ppo_xp_rnorm_step_finish_device": (_i, [_vp, _vp, _vp, _vp, _sz, _vp]),
     "ppo_xp_rnorm_state": (_i, [_vp, C.POINTER(_f), C.POINTER(_f), C.POINTER(_f), _vp, _sz]),
+    "ppo_xp_shape_logits": (_i, [_i, _vp, _i, _vp, _i64, _vp, _i64, _sz, _sz, _vp]),
+    "ppo_xp_shape_logits_backward": (_i, [_i, _vp, _i, _vp, _i64, _vp, _i64, _vp, _i64, _sz, _sz, _vp]),
+    "ppo_xp_action_stats": (_i, [_i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _sz, _sz, _vp, _sz]),
+    "ppo_xp_policy_workspace": (_sz, [_i, _sz, _sz]),
+    "ppo_xp_policy_loss": (_i, [_i, _vp, _i, _vp, _i64, _vp, _f, _f, _f, _d, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz]),
+    "ppo_xp_quantize_rows": (_i, [_i, _vp, _i, _vp, _i64, _sz, _sz, _i, _sz, _vp, _i64, _vp, _i64, _sz, _sz]),
+    "ppo_xp_dequantize_rows": (_i, [_i, _vp, _i, _vp, _i64, _vp, _i64, _sz, _sz, _i, _sz, _vp, _i, _sz, _sz, _vp, _i64]),
     "ppo_xp_stream": (_vp, [_vp]),
     "ppo_xp_set_stream": (_i, [_vp, _vp]),
     "ppo_xp_sync": (_i, [_vp]),

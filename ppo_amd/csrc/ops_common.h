@@ -1,0 +1,112 @@
+// Shared pieces of the token-policy operators (policy.hip, qrows.hip): element types, 8-wide unaligned loads and stores,
+// wave reductions, and the host side's checks.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/ppo_xp.h"
+#include "errors.h"
+
+namespace ppoxp_ops {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+// gfx950 global memory takes 16-byte accesses at any element address: rows of odd length need no peeling
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+
+// Eight consecutive elements as they lie in memory, and as floats.
+template <typename T>
+struct Raw8;
+
+template <>
+struct Raw8<float> {
+  u32x4 lo, hi;
+  __device__ __forceinline__ void load(const float *p) { lo = *(const u32x4_a4 *)p; hi = *(const u32x4_a4 *)(p + 4); }
+  __device__ __forceinline__ float get(int i) const { return __builtin_bit_cast(float, i < 4 ? lo[i & 3] : hi[i & 3]); }
+  __device__ __forceinline__ void set(int i, float x) {
+    if (i < 4) lo[i & 3] = __builtin_bit_cast(unsigned, x);
+    else hi[i & 3] = __builtin_bit_cast(unsigned, x);
+  }
+  __device__ __forceinline__ void store(float *p) const { *(u32x4_a4 *)p = lo; *(u32x4_a4 *)(p + 4) = hi; }
+};
+
+template <typename T>   // 16-bit elements: two to a register
+struct Raw8 {
+  u32x4 v;
+  __device__ __forceinline__ void load(const T *p) { v = *(const u32x4_a2 *)p; }
+  __device__ __forceinline__ float get(int i) const {
+    const unsigned short h = (unsigned short)(v[i >> 1] >> ((i & 1) * 16));
+    return (float)__builtin_bit_cast(T, h);
+  }
+  __device__ __forceinline__ void set(int i, float x) {
+    const unsigned h = __builtin_bit_cast(unsigned short, (T)x);
+    v[i >> 1] = (i & 1) ? ((v[i >> 1] & 0xffffu) | (h << 16)) : ((v[i >> 1] & 0xffff0000u) | h);
+  }
+  __device__ __forceinline__ void store(T *p) const { *(u32x4_a2 *)p = v; }
+};
+
+// The same with the end of the row in sight: elements at or beyond `left` read as `fill` and are not written.
+template <typename T>
+__device__ __forceinline__ void load8(Raw8<T> &r, const T *p, long left, float fill) {
+  if (left >= 8) { r.load(p); return; }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.set(i, i < left ? (float)p[i] : fill);
+}
+template <typename T>
+__device__ __forceinline__ void store8(const Raw8<T> &r, T *p, long left) {
+  if (left >= 8) { r.store(p); return; }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < left) p[i] = (T)r.get(i);
+}
+
+__device__ __forceinline__ float wave_max_nan(float x) {   // a NaN anywhere makes the result NaN
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x = __builtin_elementwise_maximum(x, __shfl_xor(x, off, 64));
+  return x;
+}
+template <typename F>
+__device__ __forceinline__ F wave_sum(F x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+
+// Makes `device` current for a call and puts the caller's device back.
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(int device, const char *who) {
+    int n = 0;
+    if (hipGetDevice(&prev_) != hipSuccess || (device != prev_ && (hipGetDeviceCount(&n) != hipSuccess || device < 0 || device >= n))) {
+      prev_ = -1;
+      rc_ = ppoxp_fail(PPO_XP_ENODEV, "%s: no HIP device %d (this library has no CPU path)", who, device);
+      return;
+    }
+    if (device == prev_) { prev_ = -1; return; }
+    hipError_t e = hipSetDevice(device);
+    if (e != hipSuccess) { prev_ = -1; rc_ = ppoxp_fail(PPO_XP_EIO, "%s: hipSetDevice(%d): %s", who, device, hipGetErrorString(e)); }
+  }
+  ~DeviceGuard() { if (prev_ >= 0) (void)hipSetDevice(prev_); }
+  DeviceGuard(const DeviceGuard &) = delete;
+  DeviceGuard &operator=(const DeviceGuard &) = delete;
+  int rc() const { return rc_; }
+
+ private:
+  int prev_ = -1, rc_ = 0;
+};
+
+inline int launched(const char *who) {
+  hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : ppoxp_fail(PPO_XP_EIO, "%s: launch failed: %s", who, hipGetErrorString(e));
+}
+
+inline bool is_dtype(int d) { return d == PPO_XP_F32 || d == PPO_XP_BF16 || d == PPO_XP_F16; }
+inline size_t dtype_bytes(int d) { return d == PPO_XP_F32 ? 4 : 2; }
+constexpr size_t kMaxGrid = 0x7fffffff;
+constexpr size_t kMaxVocab = size_t(1) << 30;
+
+}  // namespace ppoxp_ops
