@@ -30,6 +30,11 @@ struct Raw8<float> {
     else hi[i & 3] = __builtin_bit_cast(unsigned, x);
   }
   __device__ __forceinline__ void store(float *p) const { *(u32x4_a4 *)p = lo; *(u32x4_a4 *)(p + 4) = hi; }
+  __device__ __forceinline__ void set8(const float y[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) set(i, y[i]);
+  }
+  __device__ __forceinline__ void fill(float x) { lo = hi = u32x4(__builtin_bit_cast(unsigned, x)); }
 };
 
 template <typename T>   // 16-bit elements: two to a register
@@ -45,6 +50,15 @@ struct Raw8 {
     v[i >> 1] = (i & 1) ? ((v[i >> 1] & 0xffffu) | (h << 16)) : ((v[i >> 1] & 0xffff0000u) | h);
   }
   __device__ __forceinline__ void store(T *p) const { *(u32x4_a2 *)p = v; }
+  __device__ __forceinline__ void set8(const float y[8]) {
+    typedef T pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const pair q = {(T)y[2 * i], (T)y[2 * i + 1]};
+      v[i] = __builtin_bit_cast(unsigned, q);
+    }
+  }
+  __device__ __forceinline__ void fill(float x) { v = u32x4((unsigned)__builtin_bit_cast(unsigned short, (T)x) * 0x10001u); }
 };
 
 // The same with the end of the row in sight: elements at or beyond `left` read as `fill` and are not written.

@@ -128,7 +128,8 @@ struct PolicyArgs {
   void *dlogits;
   int64_t dstride;
   float *dvalues;
-  double *partials;      // [rows][5]: policy, value, entropy, kl, clipped
+  double *partials;      // [5][records]: policy, value, entropy, kl, clipped
+  unsigned *ticket;      // of policy_stats_kernel; the launch before it sets it to 0
 };
 
 // m = max l, s = sum e^(l-m), t = sum e^(l-m) (l-m)
@@ -169,10 +170,10 @@ __device__ __forceinline__ RowTerms row_terms(const Softmax &w, int64_t action, 
   return o;
 }
 
-// The row's share of the objective; `g` = d(policy term) / d(neglogp).
-__device__ __forceinline__ float row_objective(const PolicyArgs &a, size_t row, const RowTerms &o, double part[5]) {
+// The row's share of the objective; returns g = d(policy term) / d(neglogp).  `write`: this lane stores the value's gradient.
+__device__ __forceinline__ float row_objective(const PolicyArgs &a, size_t row, const RowTerms &o, double part[5], bool write) {
   if (o.padding) {
-    a.dvalues[row] = 0.f;
+    if (write) a.dvalues[row] = 0.f;
     for (int i = 0; i < 5; ++i) part[i] = 0.;
     return 0.f;
   }
@@ -186,7 +187,7 @@ __device__ __forceinline__ float row_objective(const PolicyArgs &a, size_t row, 
   const float e1 = v - ret, e2 = v0 + (dvv < -a.clip ? -a.clip : (dvv > a.clip ? a.clip : dvv)) - ret;
   const float q1 = e1 * e1, q2 = e2 * e2;
   const float dv = q2 > q1 ? (__builtin_fabsf(dvv) <= a.clip ? e2 : 0.f) : e1;
-  a.dvalues[row] = a.vf_coef * a.inv_denom * dv;
+  if (write) a.dvalues[row] = a.vf_coef * a.inv_denom * dv;
   const float kl = o.nlp - old;
   part[0] = plain >= clipped ? plain : (clipped > plain ? clipped : plain + clipped);
   part[1] = 0.5f * __builtin_elementwise_maximum(q1, q2);
@@ -196,110 +197,392 @@ __device__ __forceinline__ float row_objective(const PolicyArgs &a, size_t row, 
   return plain >= clipped ? A * ratio : (clipped > plain ? 0.f : plain + clipped);
 }
 
-template <int WAVES>
-__device__ __forceinline__ Softmax block_softmax(Softmax w, float *red) {   // red: 3 * WAVES floats; every thread gets the result
-  const unsigned wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const float m = wave_max_nan(w.m);
-  if (lane == 0) red[wave] = m;
-  __syncthreads();
-  float top = red[0];
-#pragma unroll
-  for (int i = 1; i < WAVES; ++i) top = __builtin_elementwise_maximum(top, red[i]);
-  rebase(w.m, top, w.s, w.t);
-  const float s = wave_sum(w.s), t = wave_sum(w.t);
-  if (lane == 0) { red[WAVES + wave] = s; red[2 * WAVES + wave] = t; }
-  __syncthreads();
-  Softmax o{top, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) { o.s += red[WAVES + i]; o.t += red[2 * WAVES + i]; }
-  return o;
+__device__ __forceinline__ void put_record(const PolicyArgs &a, size_t at, size_t records, const double part[5]) {
+  for (int i = 0; i < 5; ++i) a.partials[i * records + at] = part[i];
+  if (at == 0) *a.ticket = 0;
 }
 
+// Over the workgroup, every thread gets the result.  red: 3 * WAVES floats, a part of its own for each use.
+template <int WAVES>
+__device__ __forceinline__ float block_max(float m, float *red) {
+  m = wave_max_nan(m);
+  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = m;
+  __syncthreads();
+  m = red[0];
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) m = __builtin_elementwise_maximum(m, red[i]);
+  return m;
+}
+template <int WAVES>
+__device__ __forceinline__ void block_sums(Softmax &w, float *red) {
+  const unsigned wave = threadIdx.x / 64;
+  const float s = wave_sum(w.s), t = wave_sum(w.t);
+  if (threadIdx.x % 64 == 0) { red[WAVES + wave] = s; red[2 * WAVES + wave] = t; }
+  __syncthreads();
+  w.s = w.t = 0.f;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) { w.s += red[WAVES + i]; w.t += red[2 * WAVES + i]; }
+}
+template <int WAVES>
+__device__ __forceinline__ Softmax block_softmax(Softmax w, float *red) {
+  const float m = block_max<WAVES>(w.m, red);
+  rebase(w.m, m, w.s, w.t);
+  w.m = m;
+  block_sums<WAVES>(w, red);
+  return w;
+}
+
+// One pass with a running maximum.
 template <typename T>
-__device__ __forceinline__ void online(Softmax &w, const Raw8<T> &r, int n) {
+__device__ __forceinline__ void online(Softmax &w, const Raw8<T> &r) {
   float top = w.m;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) top = __builtin_elementwise_maximum(top, r.get(i));
+  for (int i = 0; i < 8; ++i) top = __builtin_elementwise_maximum(top, r.get(i));
   if (!(top > w.m) && w.s == 0.f) { w.m = top; return; }     // nothing but -inf so far, or NaN
   rebase(w.m, top, w.s, w.t);
   w.m = top;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) {
-      const float d = below(r.get(i), top), e = exp_neg(d);
-      w.s += e;
-      w.t = __builtin_fmaf(e, d, w.t);
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float d = below(r.get(i), top), e = exp_neg(d);
+    w.s += e;
+    w.t = __builtin_fmaf(e, d, w.t);
+  }
 }
 
-// One workgroup per row, the row read once (statistics) or twice (with the gradient, the second time out of the caches).
-template <typename T, bool LOSS>
-__global__ __launch_bounds__(256) void policy_row_kernel(PolicyArgs a) {
+// Gradient of one row's logits r (in place): dl_j = (g (p_j - 1{j = a}) + ent p_j (ln p_j + H)) / n with p_j = e_j / s and
+// ln p_j + H = d_j - t / s, so dl_j = e_j (c1 d_j + c0) - 1{j = a} g / n.
+struct GradTerms {
+  float m, c0, c1, hit;
+  bool nan, zero;
+};
+
+__device__ __forceinline__ GradTerms grad_terms(const PolicyArgs &a, float m, const RowTerms &o, float g) {
+  GradTerms k;
+  k.m = m;
+  k.c1 = o.rs * a.ent_coef * a.inv_denom;
+  k.c0 = o.rs * a.inv_denom * (g - a.ent_coef * o.t * o.rs);
+  k.hit = g * a.inv_denom;
+  k.nan = o.nan;
+  k.zero = o.padding || o.dead;
+  return k;
+}
+
+template <typename T>
+__device__ __forceinline__ void gradient8(Raw8<T> &r, const GradTerms &k, int at) {   // at: the action's place in r, if 0..7
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float d = below(r.get(i), k.m);
+    y[i] = exp_neg(d) * __builtin_fmaf(d, k.c1, k.c0);
+    if (i == at) y[i] -= k.hit;
+  }
+  if (k.nan || k.zero) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = k.zero ? 0.f : __builtin_nanf("");
+  }
+  r.set8(y);
+}
+
+// The maximum first, then the sums: rows whose elements sit in registers.  Elements beyond the row read as -inf and add nothing.
+template <typename T>
+__device__ __forceinline__ float max8(float m, const Raw8<T> &r) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = __builtin_elementwise_maximum(m, r.get(i));
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ void sums8(float m, const Raw8<T> &r, float &s, float &t) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float d = below(r.get(i), m), e = exp_neg(d);
+    s += e;
+    t = __builtin_fmaf(e, d, t);
+  }
+}
+
+// Up to kGroupVocab tokens: `lanes` neighbouring lanes of a wave hold one row in registers (8 elements and NV vectors each), so a
+// wave works on 64 / lanes rows and nothing passes through LDS.  Workgroups walk over the rows, which keeps the partial sums of
+// the objective few: one record a workgroup, added up in row order.
+constexpr unsigned kGroupVocab = 2048, kGroupBlocks = 2048;
+
+template <typename T, bool LOSS, int NV>
+__global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigned lanes_log2) {
+  __shared__ double red[4][5];
+  const unsigned lanes = 1u << lanes_log2, sub = threadIdx.x & (lanes - 1);
+  const size_t per_block = 256u >> lanes_log2;
+  double sum[5] = {0, 0, 0, 0, 0};
+  for (size_t row0 = blockIdx.x * per_block; row0 < a.rows; row0 += gridDim.x * per_block) {
+    const size_t row = row0 + (threadIdx.x >> lanes_log2);
+    const bool live = row < a.rows;
+    const T *in = (const T *)a.logits + (int64_t)row * a.stride;
+    const int64_t action = live ? a.actions[row] : -1;
+    Raw8<T> r[NV];
+    float m = -__builtin_inff();
+    if (action != -1) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) load8(r[k], in + (k * 64 + sub) * 8, (long)a.vocab - (k * 64 + sub) * 8, -__builtin_inff());
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) r[k].fill(-__builtin_inff());
+    }
+    const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) m = max8(m, r[k]);
+    for (unsigned off = 1; off < lanes; off <<= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, (int)off, 64));
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) sums8(m, r[k], s, t);
+    for (unsigned off = 1; off < lanes; off <<= 1) { s += __shfl_xor(s, (int)off, 64); t += __shfl_xor(t, (int)off, 64); }
+    if (!live) continue;
+    const RowTerms o = row_terms(Softmax{m, s, t}, action, a.vocab, l_a);
+    if (sub == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
+    if (!LOSS) continue;
+    double part[5];
+    const float g = row_objective(a, row, o, part, sub == 0);
+    if (sub == 0)
+      for (int i = 0; i < 5; ++i) sum[i] += part[i];
+    const GradTerms k = grad_terms(a, m, o, g);
+    T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const unsigned e = (v * 64 + sub) * 8;
+      if (e >= a.vocab) break;
+      gradient8(r[v], k, (int)(action - e));
+      store8(r[v], out + e, (long)(a.vocab - e));
+    }
+  }
+  if (!LOSS) return;
+  for (int i = 0; i < 5; ++i) {
+    const double x = wave_sum(sum[i]);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64][i] = x;
+  }
+  __syncthreads();
+  if (threadIdx.x < 5) a.partials[threadIdx.x * (size_t)gridDim.x + blockIdx.x] = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
+}
+
+// One workgroup per row, statistics only: the row streams through registers once.
+template <typename T>
+__global__ __launch_bounds__(256) void policy_stats_row_kernel(PolicyArgs a) {
   __shared__ float red[12];
-  __shared__ float share[4];
+  const size_t row = blockIdx.x;
+  const T *in = (const T *)a.logits + (int64_t)row * a.stride;
+  const int64_t action = a.actions[row];
+  const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
+  Softmax w{-__builtin_inff(), 0.f, 0.f};
+  if (action != -1)
+    for (unsigned e = threadIdx.x * 8; e < a.vocab; e += 2048) {
+      Raw8<T> r;
+      load8(r, in + e, (long)(a.vocab - e), -__builtin_inff());
+      online(w, r);
+    }
+  w = block_softmax<4>(w, red);
+  const RowTerms o = row_terms(w, action, a.vocab, l_a);
+  if (threadIdx.x == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
+}
+
+// One workgroup per row, the whole row in registers (NV vectors of 8 a thread): read once, the gradient written from there.
+template <typename T, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS) void policy_loss_row_kernel(PolicyArgs a) {
+  __shared__ float red[3 * THREADS / 64];
+  __shared__ float share;
   const size_t row = blockIdx.x;
   const unsigned tid = threadIdx.x;
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
   const int64_t action = a.actions[row];
-  const bool inside = action >= 0 && action < (int64_t)a.vocab;
-  const float l_a = inside ? (float)in[action] : 0.f;
+  const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
+  Raw8<T> r[NV];
   Softmax w{-__builtin_inff(), 0.f, 0.f};
-  if (action != -1)
-    for (unsigned e = tid * 8; e < a.vocab; e += 2048) {
-      Raw8<T> r;
-      load8(r, in + e, (long)(a.vocab - e), 0.f);
-      online(w, r, (int)min(8u, a.vocab - e));
-    }
-  w = block_softmax<4>(w, red);
+  if (action != -1) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) load8(r[k], in + (k * THREADS + tid) * 8, (long)a.vocab - (k * THREADS + tid) * 8, -__builtin_inff());
+#pragma unroll
+    for (int k = 0; k < NV; ++k) w.m = max8(w.m, r[k]);
+  }
+  const float m = block_max<THREADS / 64>(w.m, red);
+  if (action != -1) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) sums8(m, r[k], w.s, w.t);
+  }
+  w.m = m;
+  block_sums<THREADS / 64>(w, red);
   const RowTerms o = row_terms(w, action, a.vocab, l_a);
-  if (tid == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
-  if (!LOSS) return;
   if (tid == 0) {
+    a.neglogps[row] = o.nlp; a.entropies[row] = o.ent;
     double part[5];
-    share[0] = row_objective(a, row, o, part);
-    for (int i = 0; i < 5; ++i) a.partials[row * 5 + i] = part[i];
+    share = row_objective(a, row, o, part, true);
+    put_record(a, row, a.rows, part);
   }
   __syncthreads();
-  const float g = share[0];
+  const GradTerms k = grad_terms(a, w.m, o, share);
   T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
-  // dl_j = (g (p_j - 1{j = a}) + ent p_j (ln p_j + H)) / n,  p_j = e_j / s,  ln p_j + H = d_j - t / s
-  const float c1 = o.rs * a.ent_coef * a.inv_denom;
-  const float c0 = o.rs * a.inv_denom * (g - a.ent_coef * o.t * o.rs);
-  for (unsigned e = tid * 8; e < a.vocab; e += 2048) {
-    const int n = (int)min(8u, a.vocab - e);
-    Raw8<T> r;
-    load8(r, in + e, n, 0.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float d = below(r.get(i), w.m);
-      float y = exp_neg(d) * __builtin_fmaf(d, c1, c0);
-      if ((int64_t)(e + i) == action) y -= g * a.inv_denom;
-      if (o.nan) y = __builtin_nanf("");
-      if (o.padding || o.dead) y = 0.f;
-      r.set(i, y);
-    }
-    store8(r, out + e, n);
+  for (int v = 0; v < NV; ++v) {
+    const unsigned e = (v * THREADS + tid) * 8;
+    if (e >= a.vocab) break;
+    gradient8(r[v], k, (int)(action - e));
+    store8(r[v], out + e, (long)(a.vocab - e));
   }
 }
 
-// Sums the rows' terms in a fixed order, in 64 bits.
-__global__ __launch_bounds__(1024) void policy_stats_kernel(const double *partials, size_t n, double denom, float vf, float ent, float *stats) {
-  __shared__ double red[16][5];
-  double s[5] = {0, 0, 0, 0, 0};
-  for (size_t i = threadIdx.x; i < n; i += 1024)
-    for (int k = 0; k < 5; ++k) s[k] += partials[i * 5 + k];
+// Rows too long for the registers of a workgroup: read a second time for the gradient, out of the caches as far as they hold it.
+template <typename T>
+__global__ __launch_bounds__(1024) void policy_loss_long_kernel(PolicyArgs a) {
+  __shared__ float red[48];
+  __shared__ float share;
+  const size_t row = blockIdx.x;
+  const unsigned tid = threadIdx.x;
+  const T *in = (const T *)a.logits + (int64_t)row * a.stride;
+  const int64_t action = a.actions[row];
+  const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
+  Softmax w{-__builtin_inff(), 0.f, 0.f};
+  if (action != -1)
+    for (unsigned e = tid * 8; e < a.vocab; e += 8192) {
+      Raw8<T> r;
+      load8(r, in + e, (long)(a.vocab - e), -__builtin_inff());
+      online(w, r);
+    }
+  w = block_softmax<16>(w, red);
+  const RowTerms o = row_terms(w, action, a.vocab, l_a);
+  if (tid == 0) {
+    a.neglogps[row] = o.nlp; a.entropies[row] = o.ent;
+    double part[5];
+    share = row_objective(a, row, o, part, true);
+    put_record(a, row, a.rows, part);
+  }
+  __syncthreads();
+  const GradTerms k = grad_terms(a, w.m, o, share);
+  T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
+  for (unsigned e = tid * 8; e < a.vocab; e += 8192) {
+    Raw8<T> r;
+    load8(r, in + e, (long)(a.vocab - e), -__builtin_inff());
+    gradient8(r, k, (int)(action - e));
+    store8(r, out + e, (long)(a.vocab - e));
+  }
+}
+
+// Few long rows: every row is cut into chunks of kSplitChunk tokens, a workgroup each; the chunks' (m, s, t) meet in a second
+// launch, whose workgroups join all chunks of their row themselves.
+constexpr unsigned kSplitChunk = 4096;
+constexpr int kSplitVecs = kSplitChunk / 2048;
+
+template <typename T>
+__global__ __launch_bounds__(256) void policy_split_kernel(PolicyArgs a, unsigned chunks, Softmax *parts, float *picked) {
+  __shared__ float red[12];
+  const size_t row = blockIdx.x / chunks;
+  const unsigned c0 = (blockIdx.x % chunks) * kSplitChunk;
+  const T *in = (const T *)a.logits + (int64_t)row * a.stride;
+  Raw8<T> r[kSplitVecs];
+  Softmax w{-__builtin_inff(), 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < kSplitVecs; ++k) {
+    const unsigned e = c0 + (k * 256 + threadIdx.x) * 8;
+    load8(r[k], in + e, (long)a.vocab - (long)e, -__builtin_inff());
+  }
+#pragma unroll
+  for (int k = 0; k < kSplitVecs; ++k) w.m = max8(w.m, r[k]);
+  const float m = block_max<4>(w.m, red);
+#pragma unroll
+  for (int k = 0; k < kSplitVecs; ++k) sums8(m, r[k], w.s, w.t);
+  w.m = m;
+  block_sums<4>(w, red);
+  if (m == -__builtin_inff()) w.s = w.t = 0.f;       // -inf throughout: no terms
+  if (threadIdx.x == 0) {
+    parts[blockIdx.x] = w;
+    const int64_t action = a.actions[row];           // its logit is put aside here: the gradient may be written over the logits
+    if (action >= (int64_t)c0 && action < (int64_t)min(a.vocab, c0 + kSplitChunk)) picked[row] = (float)in[action];
+    if (blockIdx.x == 0) *a.ticket = 0;
+  }
+}
+
+__device__ __forceinline__ Softmax join_chunks(const Softmax *parts, unsigned chunks) {   // one wave, every lane gets the result
+  Softmax w{-__builtin_inff(), 0.f, 0.f};
+  for (unsigned c = threadIdx.x % 64; c < chunks; c += 64) {
+    Softmax q = parts[c];
+    const float m = __builtin_elementwise_maximum(w.m, q.m);
+    rebase(w.m, m, w.s, w.t);
+    rebase(q.m, m, q.s, q.t);
+    w = Softmax{m, w.s + q.s, w.t + q.t};
+  }
+  const float m = wave_max_nan(w.m);
+  rebase(w.m, m, w.s, w.t);
+  return Softmax{m, wave_sum(w.s), wave_sum(w.t)};
+}
+
+__global__ __launch_bounds__(64) void policy_join_kernel(PolicyArgs a, unsigned chunks, const Softmax *parts, const float *picked) {
+  const size_t row = blockIdx.x;
+  const RowTerms o = row_terms(join_chunks(parts + row * chunks, chunks), a.actions[row], a.vocab, picked[row]);
+  if (threadIdx.x == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void policy_split_loss_kernel(PolicyArgs a, unsigned chunks, const Softmax *parts, const float *picked) {
+  const size_t row = blockIdx.x / chunks;
+  const unsigned chunk = blockIdx.x % chunks, c0 = chunk * kSplitChunk, tid = threadIdx.x;
+  const T *in = (const T *)a.logits + (int64_t)row * a.stride;
+  T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
+  Raw8<T> r[kSplitVecs];
+#pragma unroll
+  for (int k = 0; k < kSplitVecs; ++k) {
+    const unsigned e = c0 + (k * 256 + tid) * 8;
+    load8(r[k], in + e, (long)a.vocab - (long)e, -__builtin_inff());
+  }
+  const int64_t action = a.actions[row];
+  const Softmax w = join_chunks(parts + row * chunks, chunks);
+  const RowTerms o = row_terms(w, action, a.vocab, picked[row]);
+  double part[5];
+  const bool first = chunk == 0 && tid == 0;
+  const float g = row_objective(a, row, o, part, first);
+  if (first) {
+    a.neglogps[row] = o.nlp; a.entropies[row] = o.ent;
+    put_record(a, row, a.rows, part);
+  }
+  const GradTerms k = grad_terms(a, w.m, o, g);
+#pragma unroll
+  for (int v = 0; v < kSplitVecs; ++v) {
+    const unsigned e = c0 + (v * 256 + tid) * 8;
+    if (e >= a.vocab) break;
+    gradient8(r[v], k, (int)(action - e));
+    store8(r[v], out + e, (long)(a.vocab - e));
+  }
+}
+
+// Sums the records in a fixed order, in 64 bits: each workgroup a slice, the last one to finish the slices.
+constexpr unsigned kStatsBlocks = 64, kStatsSlice = 1024;
+
+__device__ __forceinline__ void sum_records(const double *p, size_t stride, size_t begin, size_t end, double s[5], double (*red)[5]) {
+  for (int k = 0; k < 5; ++k) s[k] = 0;
+  for (size_t i = begin + threadIdx.x; i < end; i += 256)
+    for (int k = 0; k < 5; ++k) s[k] += p[k * stride + i];
+  __syncthreads();
   for (int k = 0; k < 5; ++k) {
     s[k] = wave_sum(s[k]);
     if (threadIdx.x % 64 == 0) red[threadIdx.x / 64][k] = s[k];
   }
   __syncthreads();
-  if (threadIdx.x) return;
-  for (int k = 0; k < 5; ++k) {
-    s[k] = 0;
-    for (int w = 0; w < 16; ++w) s[k] += red[w][k];
-    s[k] /= denom;
+  for (int k = 0; k < 5; ++k) s[k] = red[0][k] + red[1][k] + red[2][k] + red[3][k];
+}
+
+__global__ __launch_bounds__(256) void policy_stats_kernel(const double *partials, size_t n, double *slices, unsigned *ticket, double denom, float vf,
+                                                           float ent, float *stats) {
+  __shared__ double red[4][5];
+  __shared__ unsigned last;
+  double s[5];
+  const size_t per = (n + gridDim.x - 1) / gridDim.x;
+  sum_records(partials, n, min(n, blockIdx.x * per), min(n, (blockIdx.x + 1) * per), s, red);
+  if (gridDim.x > 1) {
+    if (threadIdx.x == 0) {
+      for (int k = 0; k < 5; ++k) slices[k * kStatsBlocks + blockIdx.x] = s[k];
+      __threadfence();
+      last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    sum_records(slices, kStatsBlocks, 0, gridDim.x, s, red);
   }
+  if (threadIdx.x) return;
+  for (int k = 0; k < 5; ++k) s[k] /= denom;
   stats[0] = (float)(s[0] + (double)vf * s[1] - (double)ent * s[2]);
   for (int k = 0; k < 5; ++k) stats[1 + k] = (float)s[k];
 }
@@ -374,18 +657,85 @@ int shape(const char *who, int device, void *stream, int dtype, ShapeArgs &a, si
   return launched(who);
 }
 
-template <bool LOSS>
-void launch_policy(int dtype, const PolicyArgs &a, hipStream_t s) {
-  const dim3 grid((unsigned)a.rows);
-  if (dtype == PPO_XP_F32) hipLaunchKernelGGL((policy_row_kernel<float, LOSS>), grid, dim3(256), 0, s, a);
-  else if (dtype == PPO_XP_BF16) hipLaunchKernelGGL((policy_row_kernel<__bf16, LOSS>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((policy_row_kernel<_Float16, LOSS>), grid, dim3(256), 0, s, a);
+// Which kernels a call takes, and what they need.
+enum Route { kGroup, kRow, kLong, kSplit };
+
+struct Plan {
+  Route route;
+  unsigned lanes_log2 = 0, vecs = 1, chunks = 0;   // kGroup: lanes of a row and vectors a lane; kSplit: chunks of a row
+  unsigned blocks = 0;                             // kGroup
+  size_t records = 0;                              // of the objective
+  size_t o_slices = 0, o_ticket = 0, o_parts = 0, o_picked = 0, bytes = 0;
+};
+
+// Few rows leave most of the 256 CUs idle with one workgroup each; the split costs a launch and a second read out of the caches.
+constexpr size_t kSplitRows = 256, kSplitVocab = 2 * kSplitChunk;
+constexpr size_t kRowBytes = size_t(1024) * 16 * 16;      // what 1024 threads hold in 16 vectors of 16 bytes
+
+Plan plan_of(int dtype, size_t rows, size_t vocab, bool loss) {
+  Plan p;
+  if (vocab <= kGroupVocab) {
+    p.route = kGroup;
+    while ((8u << p.lanes_log2) < vocab && p.lanes_log2 < 6) ++p.lanes_log2;
+    p.vecs = vocab <= 512 ? 1 : vocab <= 1024 ? 2 : 4;
+    const size_t per = 256u >> p.lanes_log2;
+    p.blocks = (unsigned)std::min<size_t>((rows + per - 1) / per, loss ? kGroupBlocks : kMaxGrid);
+  } else if (rows < kSplitRows && vocab >= kSplitVocab) {
+    p.route = kSplit;
+    p.chunks = (unsigned)((vocab + kSplitChunk - 1) / kSplitChunk);
+  } else {
+    p.route = !loss || vocab * dtype_bytes(dtype) <= kRowBytes ? kRow : kLong;
+  }
+  p.records = p.route == kGroup ? p.blocks : rows;
+  if (loss) p.bytes = p.records * 5 * sizeof(double);
+  p.o_slices = p.bytes;
+  if (loss) p.bytes += kStatsBlocks * 5 * sizeof(double);
+  p.o_ticket = p.bytes;
+  if (loss || p.route == kSplit) p.bytes += 16;
+  p.o_parts = p.bytes;
+  if (p.route == kSplit) p.bytes += rows * p.chunks * sizeof(Softmax);
+  p.o_picked = p.bytes;
+  if (p.route == kSplit) p.bytes += rows * sizeof(float);
+  return p;
 }
 
-int check_workspace(const char *who, int dtype, size_t rows, size_t vocab, const void *ws, size_t bytes) {
-  const size_t need = ppo_xp_policy_workspace(dtype, rows, vocab);
-  if (need && (!ws || bytes < need || (uintptr_t)ws % 16))
-    return ppoxp_fail(PPO_XP_EINVAL, "%s: workspace of %zu bytes, 16-byte aligned, expected (%zu given)", who, need, bytes);
+template <typename T, bool LOSS>
+void launch_group(const Plan &p, const PolicyArgs &a, hipStream_t s) {
+  if (p.vecs == 1) hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 1>), dim3(p.blocks), dim3(256), 0, s, a, p.lanes_log2);
+  else if (p.vecs == 2) hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 2>), dim3(p.blocks), dim3(256), 0, s, a, p.lanes_log2);
+  else hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 4>), dim3(p.blocks), dim3(256), 0, s, a, p.lanes_log2);
+}
+
+template <typename T>
+void launch_stats(const Plan &p, const PolicyArgs &a, Softmax *parts, float *picked, hipStream_t s) {
+  const unsigned rows = (unsigned)a.rows;
+  if (p.route == kGroup) launch_group<T, false>(p, a, s);
+  else if (p.route == kSplit) {
+    hipLaunchKernelGGL(policy_split_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, parts, picked);
+    hipLaunchKernelGGL(policy_join_kernel, dim3(rows), dim3(64), 0, s, a, p.chunks, (const Softmax *)parts, (const float *)picked);
+  } else hipLaunchKernelGGL(policy_stats_row_kernel<T>, dim3(rows), dim3(256), 0, s, a);
+}
+
+template <typename T>
+void launch_loss(const Plan &p, const PolicyArgs &a, Softmax *parts, float *picked, hipStream_t s) {
+  const unsigned rows = (unsigned)a.rows;
+  const size_t v16 = a.vocab * sizeof(T) / 2;            // in 16-bit elements: 8 of them or 4 floats fill 16 bytes
+  constexpr int W = sizeof(T) / 2;                       // 16-byte registers of 8 elements
+  if (p.route == kGroup) launch_group<T, true>(p, a, s);
+  else if (p.route == kSplit) {
+    hipLaunchKernelGGL(policy_split_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, parts, picked);
+    hipLaunchKernelGGL(policy_split_loss_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, (const Softmax *)parts, (const float *)picked);
+  } else if (p.route == kLong) hipLaunchKernelGGL(policy_loss_long_kernel<T>, dim3(rows), dim3(1024), 0, s, a);
+  else if (v16 <= 8192) hipLaunchKernelGGL((policy_loss_row_kernel<T, 256, 4 / W>), dim3(rows), dim3(256), 0, s, a);
+  else if (v16 <= 16384) hipLaunchKernelGGL((policy_loss_row_kernel<T, 512, 4 / W>), dim3(rows), dim3(512), 0, s, a);
+  else if (v16 <= 32768) hipLaunchKernelGGL((policy_loss_row_kernel<T, 1024, 4 / W>), dim3(rows), dim3(1024), 0, s, a);
+  else if (v16 <= 65536) hipLaunchKernelGGL((policy_loss_row_kernel<T, 1024, 8 / W>), dim3(rows), dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((policy_loss_row_kernel<T, 1024, 16 / W>), dim3(rows), dim3(1024), 0, s, a);
+}
+
+int check_workspace(const char *who, const Plan &p, const void *ws, size_t bytes) {
+  if (p.bytes && (!ws || bytes < p.bytes || (uintptr_t)ws % 16))
+    return ppoxp_fail(PPO_XP_EINVAL, "%s: workspace of %zu bytes, 16-byte aligned, expected (%zu given)", who, p.bytes, bytes);
   return 0;
 }
 
@@ -413,9 +763,8 @@ int ppo_xp_shape_logits_backward(int device, void *stream, int dtype, const void
   return shape("shape_logits_backward", device, stream, dtype, a, rows, vocab, rules, true);
 }
 
-size_t ppo_xp_policy_workspace(int dtype, size_t rows, size_t vocab) {
-  (void)dtype; (void)vocab;
-  return rows * 5 * sizeof(double);
+size_t ppo_xp_policy_workspace(int dtype, size_t rows, size_t vocab, int loss) {
+  return rows && vocab ? plan_of(dtype, rows, vocab, loss != 0).bytes : 0;
 }
 
 int ppo_xp_action_stats(int device, void *stream, int dtype, const void *logits, int64_t logits_stride, const int64_t *actions,
@@ -424,13 +773,21 @@ int ppo_xp_action_stats(int device, void *stream, int dtype, const void *logits,
   if (rows == 0 || vocab == 0) return 0;
   if (!actions || !neglogps || !entropies) return ppoxp_fail(PPO_XP_EINVAL, "action_stats: NULL argument");
   if (rows > kMaxGrid) return ppoxp_fail(PPO_XP_EINVAL, "action_stats: %zu rows are too many for one launch", rows);
-  if (int rc = check_workspace("action_stats", dtype, rows, vocab, workspace, workspace_bytes)) return rc;
+  const Plan p = plan_of(dtype, rows, vocab, false);
+  if (int rc = check_workspace("action_stats", p, workspace, workspace_bytes)) return rc;
   PolicyArgs a{};
   a.logits = logits; a.stride = logits_stride; a.actions = actions; a.neglogps = neglogps; a.entropies = entropies;
   a.vocab = (unsigned)vocab; a.rows = rows;
   DeviceGuard dev(device, "action_stats");
   if (dev.rc()) return dev.rc();
-  launch_policy<false>(dtype, a, (hipStream_t)stream);
+  char *ws = (char *)workspace;
+  a.ticket = (unsigned *)(ws + p.o_ticket);
+  Softmax *parts = (Softmax *)(ws + p.o_parts);
+  float *picked = (float *)(ws + p.o_picked);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == PPO_XP_F32) launch_stats<float>(p, a, parts, picked, s);
+  else if (dtype == PPO_XP_BF16) launch_stats<__bf16>(p, a, parts, picked, s);
+  else launch_stats<_Float16>(p, a, parts, picked, s);
   return launched("action_stats");
 }
 
@@ -447,7 +804,8 @@ int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, 
       !entropies || !stats)
     return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: NULL argument");
   if (rows > kMaxGrid) return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: %zu rows are too many for one launch", rows);
-  if (int rc = check_workspace("policy_loss", dtype, rows, vocab, workspace, workspace_bytes)) return rc;
+  const Plan p = plan_of(dtype, rows, vocab, true);
+  if (int rc = check_workspace("policy_loss", p, workspace, workspace_bytes)) return rc;
   PolicyArgs a{};
   a.logits = logits; a.stride = logits_stride; a.actions = b->actions; a.neglogps = neglogps; a.entropies = entropies;
   a.vocab = (unsigned)vocab; a.rows = rows;
@@ -456,9 +814,17 @@ int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, 
   a.dlogits = dlogits; a.dstride = dlogits_stride; a.dvalues = dvalues; a.partials = (double *)workspace;
   DeviceGuard dev(device, "policy_loss");
   if (dev.rc()) return dev.rc();
-  launch_policy<true>(dtype, a, (hipStream_t)stream);
-  if (int rc = launched("policy_loss")) return rc;
-  hipLaunchKernelGGL(policy_stats_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, (const double *)workspace, rows, denom, vf_coef, ent_coef, stats);
+  char *ws = (char *)workspace;
+  a.ticket = (unsigned *)(ws + p.o_ticket);
+  Softmax *parts = (Softmax *)(ws + p.o_parts);
+  float *picked = (float *)(ws + p.o_picked);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == PPO_XP_F32) launch_loss<float>(p, a, parts, picked, s);
+  else if (dtype == PPO_XP_BF16) launch_loss<__bf16>(p, a, parts, picked, s);
+  else launch_loss<_Float16>(p, a, parts, picked, s);
+  const unsigned slices = (unsigned)std::min<size_t>((p.records + kStatsSlice - 1) / kStatsSlice, kStatsBlocks);
+  hipLaunchKernelGGL(policy_stats_kernel, dim3(slices), dim3(256), 0, s, (const double *)a.partials, p.records, (double *)(ws + p.o_slices), a.ticket,
+                     denom, vf_coef, ent_coef, stats);
   return launched("policy_loss");
 }
 

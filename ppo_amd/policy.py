@@ -147,8 +147,8 @@ def shape_logits_backward(grad, logits, *, history=None, hist_row=None, hist_beg
     return out
 
 
-def _workspace(L, dt, rows, vocab, device):
-    n = L.ppo_xp_policy_workspace(dt, rows, vocab)
+def _workspace(L, dt, rows, vocab, loss, device):
+    n = L.ppo_xp_policy_workspace(dt, rows, vocab, loss)
     # from torch's allocator, so that calls on two streams and two captured graphs never share one
     return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
 
@@ -162,7 +162,7 @@ def action_stats(logits, actions):
     both = torch.empty(2, rows, dtype=torch.float32, device=dev)
     p = both.data_ptr()
     L, dt, d = _lib.load(), _DTYPES[logits.dtype], dev.index
-    ws, n = _workspace(L, dt, rows, vocab, dev)
+    ws, n = _workspace(L, dt, rows, vocab, 0, dev)
     check(L.ppo_xp_action_stats(d, _raw_stream(d), dt, logits.data_ptr(), stride, ap, p, p + 4 * rows, rows, vocab,
                                 ws.data_ptr() if n else None, n))
     return both[0], both[1]
@@ -194,7 +194,7 @@ def policy_loss(logits, values, batch, *, clip=0.2, ent_coef=0.01, vf_coef=0.5, 
     stats = torch.zeros(6, dtype=f32, device=dev) if rows == 0 or vocab == 0 else torch.empty(6, dtype=f32, device=dev)
     p = vec.data_ptr()
     L, dt, d = _lib.load(), _DTYPES[logits.dtype], dev.index
-    ws, n = _workspace(L, dt, rows, vocab, dev)
+    ws, n = _workspace(L, dt, rows, vocab, 1, dev)
     check(L.ppo_xp_policy_loss(d, _raw_stream(d), dt, logits.data_ptr(), stride, struct.pack("6Q", *ptrs), clip, ent_coef, vf_coef,
                                float(rows or 1) if denom is None else float(denom), dlogits.data_ptr(), dstride, p, p + 4 * rows, p + 8 * rows,
                                stats.data_ptr(), rows, vocab, ws.data_ptr() if n else None, n))

@@ -68,7 +68,7 @@ def test_backward_refusals():
 
 
 def test_stats_and_loss_refusals():
-    need = L.ppo_xp_policy_workspace(0, 4, 100)
+    need = L.ppo_xp_policy_workspace(0, 4, 100, 0)
     st = lambda dtype=0, a=P, n=P, e=P, rows=4, ws=P, nb=1 << 40: L.ppo_xp_action_stats(0, None, dtype, P, 100, a, n, e, rows, 100, ws, nb)  # noqa: E731
     refused(st(dtype=-1), "element type")
     refused(st(a=None), "NULL")
@@ -95,7 +95,7 @@ def test_stats_and_loss_refusals():
     refused(loss(ds=10), "apart")
     refused(loss(dv=None), "NULL")
     refused(loss(stats=None), "NULL")
-    need = L.ppo_xp_policy_workspace(0, 4, 100)
+    need = L.ppo_xp_policy_workspace(0, 4, 100, 1)
     assert need > 0
     refused(loss(ws=None), "workspace")
     refused(loss(nb=need - 1), "workspace")
