@@ -11,7 +11,7 @@ namespace {
 
 using namespace ppoxp_ops;
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 // ---- rules ----------------------------------------------------------------------------------------------------------------
 
@@ -132,26 +132,27 @@ struct PolicyArgs {
   unsigned *ticket;      // of policy_stats_kernel; the launch before it sets it to 0
 };
 
-// m = max l, s = sum e^(l-m), t = sum e^(l-m) (l-m)
+// A row in powers of two: m = max l, x = (l - m) log2(e), s = sum 2^x, t = sum 2^x x;  ln softmax(l)_j = ln2 (x_j - log2 s).
+// (One fma of l with a rounded m log2(e) would save an instruction, but its error grows with |m| until 2^x overflows.)
 struct Softmax { float m, s, t; };
 
-__device__ __forceinline__ float exp_neg(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }   // d <= 0
-// l - m, kept finite: e^-150 is 0 in 32 bits, and 0 * -150 is 0 where 0 * -inf is not
-__device__ __forceinline__ float below(float l, float m) { return __builtin_fmaxf(l - m, -150.f); }
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float power(float l, float m) { return (l - m) * kLog2e; }
+// ... kept finite: 2^-200 is 0 in 32 bits, and 0 * -200 is 0 where 0 * -inf is not
+__device__ __forceinline__ float finite_power(float l, float m) { return __builtin_fmaxf(power(l, m), -200.f); }
 
 // Brings (s, t) from maximum `m` to the larger or equal `to`.
 __device__ __forceinline__ void rebase(float m, float to, float &s, float &t) {
   if (s == 0.f) return;
-  const float d = below(m, to), f = exp_neg(d);
+  const float d = finite_power(m, to), f = exp2_fast(d);
   t = (t + s * d) * f;
   s *= f;
 }
 
 // What one row's statistics mean for its action.
 struct RowTerms {
-  bool padding, dead;    // dead: -inf throughout | NaN rows have nan set
-  bool nan;
-  float nlp, ent, ln_s, rs, t;
+  bool padding, dead, nan;   // dead: -inf throughout
+  float nlp, ent, rs, ts;    // rs = 1 / s, ts = t / s
 };
 
 __device__ __forceinline__ RowTerms row_terms(const Softmax &w, int64_t action, unsigned vocab, float l_a) {
@@ -162,95 +163,108 @@ __device__ __forceinline__ RowTerms row_terms(const Softmax &w, int64_t action, 
   if (o.nan) { o.nlp = o.ent = __builtin_nanf(""); return o; }
   o.dead = w.m == -__builtin_inff();
   if (o.dead) { o.nlp = __builtin_inff(); return o; }
-  o.ln_s = logf(w.s);
+  const float log2_s = log2f(w.s);
   o.rs = 1.f / w.s;
-  o.t = w.t;
-  o.nlp = o.ln_s - (l_a - w.m);
-  o.ent = o.ln_s - w.t * o.rs;
+  o.ts = w.t * o.rs;
+  o.nlp = kLn2 * (log2_s - power(l_a, w.m));
+  o.ent = kLn2 * (log2_s - o.ts);
   return o;
 }
 
-// The row's share of the objective; returns g = d(policy term) / d(neglogp).  `write`: this lane stores the value's gradient.
-__device__ __forceinline__ float row_objective(const PolicyArgs &a, size_t row, const RowTerms &o, double part[5], bool write) {
-  if (o.padding) {
-    if (write) a.dvalues[row] = 0.f;
-    for (int i = 0; i < 5; ++i) part[i] = 0.;
-    return 0.f;
-  }
-  const float A = a.advantages[row], old = a.old_neglogps[row];
-  const float v = a.values[row], v0 = a.old_values[row], ret = a.returns[row];
-  const float ratio = expf(old - o.nlp);
+// The row's entries of the batch, loaded while the logits are on their way.
+struct RowInputs { float A, old, v, v0, ret; };
+
+__device__ __forceinline__ RowInputs row_inputs(const PolicyArgs &a, size_t row) {
+  return RowInputs{a.advantages[row], a.old_neglogps[row], a.values[row], a.old_values[row], a.returns[row]};
+}
+
+// The row's share of the objective.
+struct RowShare { float g, dvalue, part[5]; };       // g = d(policy term) / d(neglogp)
+
+__device__ __forceinline__ RowShare row_objective(const PolicyArgs &a, const RowInputs &q, const RowTerms &o) {
+  RowShare r{};
+  if (o.padding) return r;
+  const float ratio = expf(q.old - o.nlp);
   const float lo = 1.f - a.clip, hi = 1.f + a.clip;
   const float held = ratio < lo ? lo : (ratio > hi ? hi : ratio);   // NaN stays NaN
-  const float plain = -A * ratio, clipped = -A * held;
-  const float dvv = v - v0;
-  const float e1 = v - ret, e2 = v0 + (dvv < -a.clip ? -a.clip : (dvv > a.clip ? a.clip : dvv)) - ret;
+  const float plain = -q.A * ratio, clipped = -q.A * held;
+  const float dvv = q.v - q.v0;
+  const float e1 = q.v - q.ret, e2 = q.v0 + (dvv < -a.clip ? -a.clip : (dvv > a.clip ? a.clip : dvv)) - q.ret;
   const float q1 = e1 * e1, q2 = e2 * e2;
-  const float dv = q2 > q1 ? (__builtin_fabsf(dvv) <= a.clip ? e2 : 0.f) : e1;
-  if (write) a.dvalues[row] = a.vf_coef * a.inv_denom * dv;
-  const float kl = o.nlp - old;
-  part[0] = plain >= clipped ? plain : (clipped > plain ? clipped : plain + clipped);
-  part[1] = 0.5f * __builtin_elementwise_maximum(q1, q2);
-  part[2] = o.ent;
-  part[3] = 0.5f * kl * kl;
-  part[4] = __builtin_fabsf(ratio - 1.f) > a.clip ? 1. : 0.;
-  return plain >= clipped ? A * ratio : (clipped > plain ? 0.f : plain + clipped);
+  const float kl = o.nlp - q.old;
+  r.dvalue = a.vf_coef * a.inv_denom * (q2 > q1 ? (__builtin_fabsf(dvv) <= a.clip ? e2 : 0.f) : e1);
+  r.part[0] = plain >= clipped ? plain : (clipped > plain ? clipped : plain + clipped);
+  r.part[1] = 0.5f * __builtin_elementwise_maximum(q1, q2);
+  r.part[2] = o.ent;
+  r.part[3] = 0.5f * kl * kl;
+  r.part[4] = __builtin_fabsf(ratio - 1.f) > a.clip ? 1.f : 0.f;
+  r.g = plain >= clipped ? q.A * ratio : (clipped > plain ? 0.f : plain + clipped);
+  return r;
 }
 
-__device__ __forceinline__ void put_record(const PolicyArgs &a, size_t at, size_t records, const double part[5]) {
-  for (int i = 0; i < 5; ++i) a.partials[i * records + at] = part[i];
-  if (at == 0) *a.ticket = 0;
+// One lane of a row's workgroup writes what the row gives.
+__device__ __forceinline__ void put_row(const PolicyArgs &a, size_t row, const RowTerms &o, const RowShare &r) {
+  a.neglogps[row] = o.nlp;
+  a.entropies[row] = o.ent;
+  a.dvalues[row] = r.dvalue;
+  for (int i = 0; i < 5; ++i) a.partials[i * a.rows + row] = r.part[i];
+  if (row == 0) *a.ticket = 0;
 }
 
-// Over the workgroup, every thread gets the result.  red: 3 * WAVES floats, a part of its own for each use.
-template <int WAVES>
+// Over a workgroup of up to 16 waves, every thread gets the result.  red: 48 floats, a third for each use.
 __device__ __forceinline__ float block_max(float m, float *red) {
   m = wave_max_nan(m);
   if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = m;
   __syncthreads();
   m = red[0];
-#pragma unroll
-  for (int i = 1; i < WAVES; ++i) m = __builtin_elementwise_maximum(m, red[i]);
+  for (unsigned i = 1; i < blockDim.x / 64; ++i) m = __builtin_elementwise_maximum(m, red[i]);
   return m;
 }
-template <int WAVES>
 __device__ __forceinline__ void block_sums(Softmax &w, float *red) {
   const unsigned wave = threadIdx.x / 64;
   const float s = wave_sum(w.s), t = wave_sum(w.t);
-  if (threadIdx.x % 64 == 0) { red[WAVES + wave] = s; red[2 * WAVES + wave] = t; }
+  if (threadIdx.x % 64 == 0) { red[16 + wave] = s; red[32 + wave] = t; }
   __syncthreads();
   w.s = w.t = 0.f;
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) { w.s += red[WAVES + i]; w.t += red[2 * WAVES + i]; }
+  for (unsigned i = 0; i < blockDim.x / 64; ++i) { w.s += red[16 + i]; w.t += red[32 + i]; }
 }
-template <int WAVES>
 __device__ __forceinline__ Softmax block_softmax(Softmax w, float *red) {
-  const float m = block_max<WAVES>(w.m, red);
+  const float m = block_max(w.m, red);
   rebase(w.m, m, w.s, w.t);
   w.m = m;
-  block_sums<WAVES>(w, red);
+  block_sums(w, red);
   return w;
+}
+
+// Elements beyond the row read as -inf and add nothing.
+template <typename T>
+__device__ __forceinline__ float max8(float m, const Raw8<T> &r) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = __builtin_elementwise_maximum(m, r.get(i));
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ void sums8(float m, const Raw8<T> &r, float &s, float &t) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = finite_power(r.get(i), m), e = exp2_fast(x);
+    s += e;
+    t = __builtin_fmaf(e, x, t);
+  }
 }
 
 // One pass with a running maximum.
 template <typename T>
 __device__ __forceinline__ void online(Softmax &w, const Raw8<T> &r) {
-  float top = w.m;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = __builtin_elementwise_maximum(top, r.get(i));
+  const float top = max8(w.m, r);
   if (!(top > w.m) && w.s == 0.f) { w.m = top; return; }     // nothing but -inf so far, or NaN
   rebase(w.m, top, w.s, w.t);
   w.m = top;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float d = below(r.get(i), top), e = exp_neg(d);
-    w.s += e;
-    w.t = __builtin_fmaf(e, d, w.t);
-  }
+  sums8(top, r, w.s, w.t);
 }
 
 // Gradient of one row's logits r (in place): dl_j = (g (p_j - 1{j = a}) + ent p_j (ln p_j + H)) / n with p_j = e_j / s and
-// ln p_j + H = d_j - t / s, so dl_j = e_j (c1 d_j + c0) - 1{j = a} g / n.
+// ln p_j + H = ln2 (x_j - t / s), so dl_j = e_j (c1 x_j + c0) - 1{j = a} g / n.
 struct GradTerms {
   float m, c0, c1, hit;
   bool nan, zero;
@@ -259,8 +273,8 @@ struct GradTerms {
 __device__ __forceinline__ GradTerms grad_terms(const PolicyArgs &a, float m, const RowTerms &o, float g) {
   GradTerms k;
   k.m = m;
-  k.c1 = o.rs * a.ent_coef * a.inv_denom;
-  k.c0 = o.rs * a.inv_denom * (g - a.ent_coef * o.t * o.rs);
+  k.c1 = o.rs * (kLn2 * a.ent_coef) * a.inv_denom;
+  k.c0 = o.rs * a.inv_denom * (g - (kLn2 * a.ent_coef) * o.ts);
   k.hit = g * a.inv_denom;
   k.nan = o.nan;
   k.zero = o.padding || o.dead;
@@ -272,32 +286,19 @@ __device__ __forceinline__ void gradient8(Raw8<T> &r, const GradTerms &k, int at
   float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float d = below(r.get(i), k.m);
-    y[i] = exp_neg(d) * __builtin_fmaf(d, k.c1, k.c0);
-    if (i == at) y[i] -= k.hit;
+    const float x = finite_power(r.get(i), k.m);
+    y[i] = exp2_fast(x) * __builtin_fmaf(x, k.c1, k.c0);
+  }
+  if ((unsigned)at < 8u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i == at) y[i] -= k.hit;
   }
   if (k.nan || k.zero) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = k.zero ? 0.f : __builtin_nanf("");
   }
   r.set8(y);
-}
-
-// The maximum first, then the sums: rows whose elements sit in registers.  Elements beyond the row read as -inf and add nothing.
-template <typename T>
-__device__ __forceinline__ float max8(float m, const Raw8<T> &r) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = __builtin_elementwise_maximum(m, r.get(i));
-  return m;
-}
-template <typename T>
-__device__ __forceinline__ void sums8(float m, const Raw8<T> &r, float &s, float &t) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float d = below(r.get(i), m), e = exp_neg(d);
-    s += e;
-    t = __builtin_fmaf(e, d, t);
-  }
 }
 
 // Up to kGroupVocab tokens: `lanes` neighbouring lanes of a wave hold one row in registers (8 elements and NV vectors each), so a
@@ -316,6 +317,8 @@ __global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigne
     const bool live = row < a.rows;
     const T *in = (const T *)a.logits + (int64_t)row * a.stride;
     const int64_t action = live ? a.actions[row] : -1;
+    RowInputs q{};
+    if (LOSS && live) q = row_inputs(a, row);
     Raw8<T> r[NV];
     float m = -__builtin_inff();
     if (action != -1) {
@@ -337,11 +340,12 @@ __global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigne
     const RowTerms o = row_terms(Softmax{m, s, t}, action, a.vocab, l_a);
     if (sub == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
     if (!LOSS) continue;
-    double part[5];
-    const float g = row_objective(a, row, o, part, sub == 0);
-    if (sub == 0)
-      for (int i = 0; i < 5; ++i) sum[i] += part[i];
-    const GradTerms k = grad_terms(a, m, o, g);
+    const RowShare share = row_objective(a, q, o);
+    if (sub == 0) {
+      a.dvalues[row] = share.dvalue;
+      for (int i = 0; i < 5; ++i) sum[i] += share.part[i];
+    }
+    const GradTerms k = grad_terms(a, m, o, share.g);
     T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -364,7 +368,7 @@ __global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigne
 // One workgroup per row, statistics only: the row streams through registers once.
 template <typename T>
 __global__ __launch_bounds__(256) void policy_stats_row_kernel(PolicyArgs a) {
-  __shared__ float red[12];
+  __shared__ float red[48];
   const size_t row = blockIdx.x;
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
   const int64_t action = a.actions[row];
@@ -376,49 +380,44 @@ __global__ __launch_bounds__(256) void policy_stats_row_kernel(PolicyArgs a) {
       load8(r, in + e, (long)(a.vocab - e), -__builtin_inff());
       online(w, r);
     }
-  w = block_softmax<4>(w, red);
+  w = block_softmax(w, red);
   const RowTerms o = row_terms(w, action, a.vocab, l_a);
   if (threadIdx.x == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
 }
 
 // One workgroup per row, the whole row in registers (NV vectors of 8 a thread): read once, the gradient written from there.
-template <typename T, int THREADS, int NV>
-__global__ __launch_bounds__(THREADS) void policy_loss_row_kernel(PolicyArgs a) {
-  __shared__ float red[3 * THREADS / 64];
-  __shared__ float share;
+// Rows of up to half the registers leave room for a second workgroup, which loads while the first computes.
+template <typename T, int NV>
+__global__ __launch_bounds__(1024, NV * sizeof(Raw8<T>) <= 128 ? 8 : 4) void policy_loss_row_kernel(PolicyArgs a) {
+  __shared__ float red[48];
   const size_t row = blockIdx.x;
-  const unsigned tid = threadIdx.x;
+  const unsigned tid = threadIdx.x, threads = blockDim.x;
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
   const int64_t action = a.actions[row];
   const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
+  const RowInputs q = row_inputs(a, row);
   Raw8<T> r[NV];
   Softmax w{-__builtin_inff(), 0.f, 0.f};
   if (action != -1) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) load8(r[k], in + (k * THREADS + tid) * 8, (long)a.vocab - (k * THREADS + tid) * 8, -__builtin_inff());
+    for (int k = 0; k < NV; ++k) load8(r[k], in + (k * threads + tid) * 8, (long)a.vocab - (k * threads + tid) * 8, -__builtin_inff());
 #pragma unroll
     for (int k = 0; k < NV; ++k) w.m = max8(w.m, r[k]);
   }
-  const float m = block_max<THREADS / 64>(w.m, red);
+  w.m = block_max(w.m, red);
   if (action != -1) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) sums8(m, r[k], w.s, w.t);
+    for (int k = 0; k < NV; ++k) sums8(w.m, r[k], w.s, w.t);
   }
-  w.m = m;
-  block_sums<THREADS / 64>(w, red);
+  block_sums(w, red);
   const RowTerms o = row_terms(w, action, a.vocab, l_a);
-  if (tid == 0) {
-    a.neglogps[row] = o.nlp; a.entropies[row] = o.ent;
-    double part[5];
-    share = row_objective(a, row, o, part, true);
-    put_record(a, row, a.rows, part);
-  }
-  __syncthreads();
-  const GradTerms k = grad_terms(a, w.m, o, share);
+  const RowShare share = row_objective(a, q, o);
+  if (tid == 0) put_row(a, row, o, share);
+  const GradTerms k = grad_terms(a, w.m, o, share.g);
   T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const unsigned e = (v * THREADS + tid) * 8;
+    const unsigned e = (v * threads + tid) * 8;
     if (e >= a.vocab) break;
     gradient8(r[v], k, (int)(action - e));
     store8(r[v], out + e, (long)(a.vocab - e));
@@ -429,12 +428,12 @@ __global__ __launch_bounds__(THREADS) void policy_loss_row_kernel(PolicyArgs a) 
 template <typename T>
 __global__ __launch_bounds__(1024) void policy_loss_long_kernel(PolicyArgs a) {
   __shared__ float red[48];
-  __shared__ float share;
   const size_t row = blockIdx.x;
   const unsigned tid = threadIdx.x;
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
   const int64_t action = a.actions[row];
   const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
+  const RowInputs q = row_inputs(a, row);
   Softmax w{-__builtin_inff(), 0.f, 0.f};
   if (action != -1)
     for (unsigned e = tid * 8; e < a.vocab; e += 8192) {
@@ -442,16 +441,11 @@ __global__ __launch_bounds__(1024) void policy_loss_long_kernel(PolicyArgs a) {
       load8(r, in + e, (long)(a.vocab - e), -__builtin_inff());
       online(w, r);
     }
-  w = block_softmax<16>(w, red);
+  w = block_softmax(w, red);
   const RowTerms o = row_terms(w, action, a.vocab, l_a);
-  if (tid == 0) {
-    a.neglogps[row] = o.nlp; a.entropies[row] = o.ent;
-    double part[5];
-    share = row_objective(a, row, o, part, true);
-    put_record(a, row, a.rows, part);
-  }
-  __syncthreads();
-  const GradTerms k = grad_terms(a, w.m, o, share);
+  const RowShare share = row_objective(a, q, o);
+  if (tid == 0) put_row(a, row, o, share);
+  const GradTerms k = grad_terms(a, w.m, o, share.g);
   T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
   for (unsigned e = tid * 8; e < a.vocab; e += 8192) {
     Raw8<T> r;
@@ -468,7 +462,7 @@ constexpr int kSplitVecs = kSplitChunk / 2048;
 
 template <typename T>
 __global__ __launch_bounds__(256) void policy_split_kernel(PolicyArgs a, unsigned chunks, Softmax *parts, float *picked) {
-  __shared__ float red[12];
+  __shared__ float red[48];
   const size_t row = blockIdx.x / chunks;
   const unsigned c0 = (blockIdx.x % chunks) * kSplitChunk;
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
@@ -481,11 +475,11 @@ __global__ __launch_bounds__(256) void policy_split_kernel(PolicyArgs a, unsigne
   }
 #pragma unroll
   for (int k = 0; k < kSplitVecs; ++k) w.m = max8(w.m, r[k]);
-  const float m = block_max<4>(w.m, red);
+  const float m = block_max(w.m, red);
 #pragma unroll
   for (int k = 0; k < kSplitVecs; ++k) sums8(m, r[k], w.s, w.t);
   w.m = m;
-  block_sums<4>(w, red);
+  block_sums(w, red);
   if (m == -__builtin_inff()) w.s = w.t = 0.f;       // -inf throughout: no terms
   if (threadIdx.x == 0) {
     parts[blockIdx.x] = w;
@@ -527,17 +521,13 @@ __global__ __launch_bounds__(256) void policy_split_loss_kernel(PolicyArgs a, un
     const unsigned e = c0 + (k * 256 + tid) * 8;
     load8(r[k], in + e, (long)a.vocab - (long)e, -__builtin_inff());
   }
+  const RowInputs q = row_inputs(a, row);
   const int64_t action = a.actions[row];
   const Softmax w = join_chunks(parts + row * chunks, chunks);
   const RowTerms o = row_terms(w, action, a.vocab, picked[row]);
-  double part[5];
-  const bool first = chunk == 0 && tid == 0;
-  const float g = row_objective(a, row, o, part, first);
-  if (first) {
-    a.neglogps[row] = o.nlp; a.entropies[row] = o.ent;
-    put_record(a, row, a.rows, part);
-  }
-  const GradTerms k = grad_terms(a, w.m, o, g);
+  const RowShare share = row_objective(a, q, o);
+  if (chunk == 0 && tid == 0) put_row(a, row, o, share);
+  const GradTerms k = grad_terms(a, w.m, o, share.g);
 #pragma unroll
   for (int v = 0; v < kSplitVecs; ++v) {
     const unsigned e = c0 + (v * 256 + tid) * 8;
@@ -547,25 +537,25 @@ __global__ __launch_bounds__(256) void policy_split_loss_kernel(PolicyArgs a, un
   }
 }
 
-// Sums the records in a fixed order, in 64 bits: each workgroup a slice, the last one to finish the slices.
-constexpr unsigned kStatsBlocks = 64, kStatsSlice = 1024;
+// Sums the records in a fixed order, in 64 bits: each workgroup a slice, three waves a column; the last workgroup to finish adds
+// the slices.
+constexpr unsigned kStatsBlocks = 64, kStatsSlice = 8192;
 
-__device__ __forceinline__ void sum_records(const double *p, size_t stride, size_t begin, size_t end, double s[5], double (*red)[5]) {
-  for (int k = 0; k < 5; ++k) s[k] = 0;
-  for (size_t i = begin + threadIdx.x; i < end; i += 256)
-    for (int k = 0; k < 5; ++k) s[k] += p[k * stride + i];
+__device__ __forceinline__ void sum_records(const double *p, size_t stride, size_t begin, size_t end, double s[5], double *red) {
+  const unsigned wave = threadIdx.x / 64, column = wave / 3;
+  double x = 0;
+#pragma unroll 8
+  for (size_t i = begin + (wave % 3) * 64 + threadIdx.x % 64; i < end; i += 192) x += p[column * stride + i];
+  x = wave_sum(x);
   __syncthreads();
-  for (int k = 0; k < 5; ++k) {
-    s[k] = wave_sum(s[k]);
-    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64][k] = s[k];
-  }
+  if (threadIdx.x % 64 == 0) red[wave] = x;
   __syncthreads();
-  for (int k = 0; k < 5; ++k) s[k] = red[0][k] + red[1][k] + red[2][k] + red[3][k];
+  for (int k = 0; k < 5; ++k) s[k] = red[3 * k] + red[3 * k + 1] + red[3 * k + 2];
 }
 
-__global__ __launch_bounds__(256) void policy_stats_kernel(const double *partials, size_t n, double *slices, unsigned *ticket, double denom, float vf,
+__global__ __launch_bounds__(960) void policy_stats_kernel(const double *partials, size_t n, double *slices, unsigned *ticket, double denom, float vf,
                                                            float ent, float *stats) {
-  __shared__ double red[4][5];
+  __shared__ double red[15];
   __shared__ unsigned last;
   double s[5];
   const size_t per = (n + gridDim.x - 1) / gridDim.x;
@@ -716,21 +706,27 @@ void launch_stats(const Plan &p, const PolicyArgs &a, Softmax *parts, float *pic
   } else hipLaunchKernelGGL(policy_stats_row_kernel<T>, dim3(rows), dim3(256), 0, s, a);
 }
 
+// The fewest vectors a thread that let 1024 threads hold the row (half a kRowBytes row and more take steps of two), and no more
+// threads than that needs.
+template <typename T, int NV>
+void launch_row(const PolicyArgs &a, unsigned vecs, hipStream_t s) {
+  constexpr int kMost = 16 / (sizeof(T) / 2), kStep = NV >= 8 ? 2 : 1;
+  if constexpr (NV < kMost) {
+    if (vecs > NV * 1024u) return launch_row<T, NV + kStep>(a, vecs, s);
+  }
+  const unsigned threads = ((vecs + NV - 1) / NV + 63) / 64 * 64;
+  hipLaunchKernelGGL((policy_loss_row_kernel<T, NV>), dim3((unsigned)a.rows), dim3(threads), 0, s, a);
+}
+
 template <typename T>
 void launch_loss(const Plan &p, const PolicyArgs &a, Softmax *parts, float *picked, hipStream_t s) {
   const unsigned rows = (unsigned)a.rows;
-  const size_t v16 = a.vocab * sizeof(T) / 2;            // in 16-bit elements: 8 of them or 4 floats fill 16 bytes
-  constexpr int W = sizeof(T) / 2;                       // 16-byte registers of 8 elements
   if (p.route == kGroup) launch_group<T, true>(p, a, s);
   else if (p.route == kSplit) {
     hipLaunchKernelGGL(policy_split_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, parts, picked);
     hipLaunchKernelGGL(policy_split_loss_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, (const Softmax *)parts, (const float *)picked);
   } else if (p.route == kLong) hipLaunchKernelGGL(policy_loss_long_kernel<T>, dim3(rows), dim3(1024), 0, s, a);
-  else if (v16 <= 8192) hipLaunchKernelGGL((policy_loss_row_kernel<T, 256, 4 / W>), dim3(rows), dim3(256), 0, s, a);
-  else if (v16 <= 16384) hipLaunchKernelGGL((policy_loss_row_kernel<T, 512, 4 / W>), dim3(rows), dim3(512), 0, s, a);
-  else if (v16 <= 32768) hipLaunchKernelGGL((policy_loss_row_kernel<T, 1024, 4 / W>), dim3(rows), dim3(1024), 0, s, a);
-  else if (v16 <= 65536) hipLaunchKernelGGL((policy_loss_row_kernel<T, 1024, 8 / W>), dim3(rows), dim3(1024), 0, s, a);
-  else hipLaunchKernelGGL((policy_loss_row_kernel<T, 1024, 16 / W>), dim3(rows), dim3(1024), 0, s, a);
+  else launch_row<T, 8 / sizeof(T)>(a, (a.vocab + 7) / 8, s);
 }
 
 int check_workspace(const char *who, const Plan &p, const void *ws, size_t bytes) {
@@ -823,7 +819,7 @@ int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, 
   else if (dtype == PPO_XP_BF16) launch_loss<__bf16>(p, a, parts, picked, s);
   else launch_loss<_Float16>(p, a, parts, picked, s);
   const unsigned slices = (unsigned)std::min<size_t>((p.records + kStatsSlice - 1) / kStatsSlice, kStatsBlocks);
-  hipLaunchKernelGGL(policy_stats_kernel, dim3(slices), dim3(256), 0, s, (const double *)a.partials, p.records, (double *)(ws + p.o_slices), a.ticket,
+  hipLaunchKernelGGL(policy_stats_kernel, dim3(slices), dim3(960), 0, s, (const double *)a.partials, p.records, (double *)(ws + p.o_slices), a.ticket,
                      denom, vf_coef, ent_coef, stats);
   return launched("policy_loss");
 }
