@@ -35,6 +35,7 @@ struct Raw8<float> {
     for (int i = 0; i < 8; ++i) set(i, y[i]);
   }
   __device__ __forceinline__ void fill(float x) { lo = hi = u32x4(__builtin_bit_cast(unsigned, x)); }
+  __device__ __forceinline__ void pin() {}
 };
 
 template <typename T>   // 16-bit elements: two to a register
@@ -59,6 +60,8 @@ struct Raw8 {
     }
   }
   __device__ __forceinline__ void fill(float x) { v = u32x4((unsigned)__builtin_bit_cast(unsigned short, (T)x) * 0x10001u); }
+  // Forgets what the elements are as floats: converting them once more is an instruction, keeping them takes twice the registers.
+  __device__ __forceinline__ void pin() { asm volatile("" : "+v"(v)); }
 };
 
 // The same with the end of the row in sight: elements at or beyond `left` read as `fill` and are not written.
@@ -76,13 +79,34 @@ __device__ __forceinline__ void store8(const Raw8<T> &r, T *p, long left) {
     if (i < left) p[i] = (T)r.get(i);
 }
 
-__device__ __forceinline__ float wave_max_nan(float x) {   // a NaN anywhere makes the result NaN
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x = __builtin_elementwise_maximum(x, __shfl_xor(x, off, 64));
-  return x;
+// Wave reductions in the vector unit (rotations within 16 lanes, then the row broadcasts): lane 63 ends with the whole wave's
+// value, which every lane gets.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float other, float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, other), __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
 }
-template <typename F>
-__device__ __forceinline__ F wave_sum(F x) {
+__device__ __forceinline__ float last_lane(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ float wave_max_nan(float x) {   // a NaN anywhere makes the result NaN
+  x = __builtin_elementwise_maximum(x, dpp<0x128, 0xf>(x, x));
+  x = __builtin_elementwise_maximum(x, dpp<0x124, 0xf>(x, x));
+  x = __builtin_elementwise_maximum(x, dpp<0x122, 0xf>(x, x));
+  x = __builtin_elementwise_maximum(x, dpp<0x121, 0xf>(x, x));
+  x = __builtin_elementwise_maximum(x, dpp<0x142, 0xa>(x, x));
+  x = __builtin_elementwise_maximum(x, dpp<0x143, 0xc>(x, x));
+  return last_lane(x);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x += dpp<0x128, 0xf>(0.f, x);
+  x += dpp<0x124, 0xf>(0.f, x);
+  x += dpp<0x122, 0xf>(0.f, x);
+  x += dpp<0x121, 0xf>(0.f, x);
+  x += dpp<0x142, 0xa>(0.f, x);
+  x += dpp<0x143, 0xc>(0.f, x);
+  return last_lane(x);
+}
+__device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
   return x;

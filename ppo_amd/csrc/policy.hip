@@ -211,29 +211,20 @@ __device__ __forceinline__ void put_row(const PolicyArgs &a, size_t row, const R
   if (row == 0) *a.ticket = 0;
 }
 
-// Over a workgroup of up to 16 waves, every thread gets the result.  red: 48 floats, a third for each use.
-__device__ __forceinline__ float block_max(float m, float *red) {
-  m = wave_max_nan(m);
-  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = m;
-  __syncthreads();
-  m = red[0];
-  for (unsigned i = 1; i < blockDim.x / 64; ++i) m = __builtin_elementwise_maximum(m, red[i]);
-  return m;
-}
-__device__ __forceinline__ void block_sums(Softmax &w, float *red) {
-  const unsigned wave = threadIdx.x / 64;
-  const float s = wave_sum(w.s), t = wave_sum(w.t);
-  if (threadIdx.x % 64 == 0) { red[16 + wave] = s; red[32 + wave] = t; }
-  __syncthreads();
-  w.s = w.t = 0.f;
-  for (unsigned i = 0; i < blockDim.x / 64; ++i) { w.s += red[16 + i]; w.t += red[32 + i]; }
-}
-__device__ __forceinline__ Softmax block_softmax(Softmax w, float *red) {
-  const float m = block_max(w.m, red);
+// Joins the lanes' statistics, each relative to its own maximum, over a workgroup of up to 16 waves with one barrier; every
+// thread gets the result.  A maximum of NaN stays NaN.
+__device__ __forceinline__ Softmax wave_softmax(Softmax w) {
+  const float m = wave_max_nan(w.m);
   rebase(w.m, m, w.s, w.t);
-  w.m = m;
-  block_sums(w, red);
-  return w;
+  return Softmax{m, wave_sum(w.s), wave_sum(w.t)};
+}
+__device__ __forceinline__ Softmax block_softmax(Softmax w, Softmax *red) {   // red: 16
+  w = wave_softmax(w);
+  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = w;
+  __syncthreads();
+  const unsigned lane = threadIdx.x % 64;
+  w = lane < blockDim.x / 64 ? red[lane] : Softmax{-__builtin_inff(), 0.f, 0.f};
+  return wave_softmax(w);
 }
 
 // Elements beyond the row read as -inf and add nothing.
@@ -250,6 +241,20 @@ __device__ __forceinline__ void sums8(float m, const Raw8<T> &r, float &s, float
     const float x = finite_power(r.get(i), m), e = exp2_fast(x);
     s += e;
     t = __builtin_fmaf(e, x, t);
+  }
+}
+
+// Vectors that sit in registers.
+template <int NV, typename T>
+__device__ __forceinline__ void row_softmax(Softmax &w, Raw8<T> *r) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) w.m = max8(w.m, r[k]);
+  if (w.m == -__builtin_inff()) return;                       // -inf throughout: no terms
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    r[k].pin();
+    sums8(w.m, r[k], w.s, w.t);
+    r[k].pin();
   }
 }
 
@@ -368,7 +373,7 @@ __global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigne
 // One workgroup per row, statistics only: the row streams through registers once.
 template <typename T>
 __global__ __launch_bounds__(256) void policy_stats_row_kernel(PolicyArgs a) {
-  __shared__ float red[48];
+  __shared__ Softmax red[16];
   const size_t row = blockIdx.x;
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
   const int64_t action = a.actions[row];
@@ -389,7 +394,7 @@ __global__ __launch_bounds__(256) void policy_stats_row_kernel(PolicyArgs a) {
 // Rows of up to half the registers leave room for a second workgroup, which loads while the first computes.
 template <typename T, int NV>
 __global__ __launch_bounds__(1024, NV * sizeof(Raw8<T>) <= 128 ? 8 : 4) void policy_loss_row_kernel(PolicyArgs a) {
-  __shared__ float red[48];
+  __shared__ Softmax red[16];
   const size_t row = blockIdx.x;
   const unsigned tid = threadIdx.x, threads = blockDim.x;
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
@@ -401,15 +406,9 @@ __global__ __launch_bounds__(1024, NV * sizeof(Raw8<T>) <= 128 ? 8 : 4) void pol
   if (action != -1) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) load8(r[k], in + (k * threads + tid) * 8, (long)a.vocab - (k * threads + tid) * 8, -__builtin_inff());
-#pragma unroll
-    for (int k = 0; k < NV; ++k) w.m = max8(w.m, r[k]);
+    row_softmax<NV>(w, r);
   }
-  w.m = block_max(w.m, red);
-  if (action != -1) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) sums8(w.m, r[k], w.s, w.t);
-  }
-  block_sums(w, red);
+  w = block_softmax(w, red);
   const RowTerms o = row_terms(w, action, a.vocab, l_a);
   const RowShare share = row_objective(a, q, o);
   if (tid == 0) put_row(a, row, o, share);
@@ -427,7 +426,7 @@ __global__ __launch_bounds__(1024, NV * sizeof(Raw8<T>) <= 128 ? 8 : 4) void pol
 // Rows too long for the registers of a workgroup: read a second time for the gradient, out of the caches as far as they hold it.
 template <typename T>
 __global__ __launch_bounds__(1024) void policy_loss_long_kernel(PolicyArgs a) {
-  __shared__ float red[48];
+  __shared__ Softmax red[16];
   const size_t row = blockIdx.x;
   const unsigned tid = threadIdx.x;
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
@@ -462,7 +461,7 @@ constexpr int kSplitVecs = kSplitChunk / 2048;
 
 template <typename T>
 __global__ __launch_bounds__(256) void policy_split_kernel(PolicyArgs a, unsigned chunks, Softmax *parts, float *picked) {
-  __shared__ float red[48];
+  __shared__ Softmax red[16];
   const size_t row = blockIdx.x / chunks;
   const unsigned c0 = (blockIdx.x % chunks) * kSplitChunk;
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
@@ -473,14 +472,8 @@ __global__ __launch_bounds__(256) void policy_split_kernel(PolicyArgs a, unsigne
     const unsigned e = c0 + (k * 256 + threadIdx.x) * 8;
     load8(r[k], in + e, (long)a.vocab - (long)e, -__builtin_inff());
   }
-#pragma unroll
-  for (int k = 0; k < kSplitVecs; ++k) w.m = max8(w.m, r[k]);
-  const float m = block_max(w.m, red);
-#pragma unroll
-  for (int k = 0; k < kSplitVecs; ++k) sums8(m, r[k], w.s, w.t);
-  w.m = m;
-  block_sums(w, red);
-  if (m == -__builtin_inff()) w.s = w.t = 0.f;       // -inf throughout: no terms
+  row_softmax<kSplitVecs>(w, r);
+  w = block_softmax(w, red);
   if (threadIdx.x == 0) {
     parts[blockIdx.x] = w;
     const int64_t action = a.actions[row];           // its logit is put aside here: the gradient may be written over the logits
@@ -498,9 +491,7 @@ __device__ __forceinline__ Softmax join_chunks(const Softmax *parts, unsigned ch
     rebase(q.m, m, q.s, q.t);
     w = Softmax{m, w.s + q.s, w.t + q.t};
   }
-  const float m = wave_max_nan(w.m);
-  rebase(w.m, m, w.s, w.t);
-  return Softmax{m, wave_sum(w.s), wave_sum(w.t)};
+  return wave_softmax(w);
 }
 
 __global__ __launch_bounds__(64) void policy_join_kernel(PolicyArgs a, unsigned chunks, const Softmax *parts, const float *picked) {
@@ -706,16 +697,36 @@ void launch_stats(const Plan &p, const PolicyArgs &a, Softmax *parts, float *pic
   } else hipLaunchKernelGGL(policy_stats_row_kernel<T>, dim3(rows), dim3(256), 0, s, a);
 }
 
-// The fewest vectors a thread that let 1024 threads hold the row (half a kRowBytes row and more take steps of two), and no more
-// threads than that needs.
+// Vectors a thread: the choice that keeps most rows in a CU at once, whose phases then overlap; of equal ones the smallest.
+// `kWaves`: waves a CU holds of the kernel with that many vectors (its registers: 24 and 4 a vector, 8 of floats).
+constexpr int row_waves(int regs) { return 512 / ((regs + 7) / 8 * 8) >= 8 ? 32 : 512 / ((regs + 7) / 8 * 8) * 4; }
+
 template <typename T, int NV>
-void launch_row(const PolicyArgs &a, unsigned vecs, hipStream_t s) {
-  constexpr int kMost = 16 / (sizeof(T) / 2), kStep = NV >= 8 ? 2 : 1;
-  if constexpr (NV < kMost) {
-    if (vecs > NV * 1024u) return launch_row<T, NV + kStep>(a, vecs, s);
-  }
+void launch_row_as(const PolicyArgs &a, unsigned vecs, hipStream_t s) {
   const unsigned threads = ((vecs + NV - 1) / NV + 63) / 64 * 64;
   hipLaunchKernelGGL((policy_loss_row_kernel<T, NV>), dim3((unsigned)a.rows), dim3(threads), 0, s, a);
+}
+
+template <typename T>
+void launch_row(const PolicyArgs &a, hipStream_t s) {
+  constexpr int kScale = sizeof(T) / 2;                 // 16-byte registers of 8 elements
+  static const int choices[] = {4, 6, 8, 10, 12, 14, 16};
+  const unsigned vecs = (a.vocab + 7) / 8;
+  int best = 0, rows = 0;
+  for (int c : choices) {
+    const unsigned waves = (vecs + c / kScale * 64 - 1) / (c / kScale * 64);
+    const int held = waves <= 16 ? row_waves(28 + 4 * c) / (int)waves : 0;
+    if (held > rows) { rows = held; best = c; }
+  }
+  switch (best) {
+    case 4: launch_row_as<T, 4 / kScale>(a, vecs, s); break;
+    case 6: launch_row_as<T, 6 / kScale>(a, vecs, s); break;
+    case 8: launch_row_as<T, 8 / kScale>(a, vecs, s); break;
+    case 10: launch_row_as<T, 10 / kScale>(a, vecs, s); break;
+    case 12: launch_row_as<T, 12 / kScale>(a, vecs, s); break;
+    case 14: launch_row_as<T, 14 / kScale>(a, vecs, s); break;
+    default: launch_row_as<T, 16 / kScale>(a, vecs, s); break;
+  }
 }
 
 template <typename T>
@@ -726,7 +737,7 @@ void launch_loss(const Plan &p, const PolicyArgs &a, Softmax *parts, float *pick
     hipLaunchKernelGGL(policy_split_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, parts, picked);
     hipLaunchKernelGGL(policy_split_loss_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, (const Softmax *)parts, (const float *)picked);
   } else if (p.route == kLong) hipLaunchKernelGGL(policy_loss_long_kernel<T>, dim3(rows), dim3(1024), 0, s, a);
-  else launch_row<T, 8 / sizeof(T)>(a, (a.vocab + 7) / 8, s);
+  else launch_row<T>(a, s);
 }
 
 int check_workspace(const char *who, const Plan &p, const void *ws, size_t bytes) {
