@@ -35,7 +35,7 @@ struct Raw8<float> {
     for (int i = 0; i < 8; ++i) set(i, y[i]);
   }
   __device__ __forceinline__ void fill(float x) { lo = hi = u32x4(__builtin_bit_cast(unsigned, x)); }
-  __device__ __forceinline__ void pin() {}
+  __device__ __forceinline__ float fresh(int i) const { return get(i); }
 };
 
 template <typename T>   // 16-bit elements: two to a register
@@ -60,16 +60,36 @@ struct Raw8 {
     }
   }
   __device__ __forceinline__ void fill(float x) { v = u32x4((unsigned)__builtin_bit_cast(unsigned short, (T)x) * 0x10001u); }
-  // Forgets what the elements are as floats: converting them once more is an instruction, keeping them takes twice the registers.
-  __device__ __forceinline__ void pin() { asm volatile("" : "+v"(v)); }
+  // get() that is computed here and now: left to itself the compiler keeps the floats of an earlier use, twice the registers.
+  __device__ __forceinline__ float fresh(int i) const {
+    float x;
+    const unsigned w = v[i >> 1];
+    if constexpr (__is_same(T, __bf16)) {
+      if (i & 1) asm volatile("v_and_b32 %0, 0xffff0000, %1" : "=v"(x) : "v"(w));
+      else asm volatile("v_lshlrev_b32 %0, 16, %1" : "=v"(x) : "v"(w));
+    } else {
+      if (i & 1) asm volatile("v_cvt_f32_f16_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_1" : "=v"(x) : "v"(w));
+      else asm volatile("v_cvt_f32_f16 %0, %1" : "=v"(x) : "v"(w));
+    }
+    return x;
+  }
 };
 
-// The same with the end of the row in sight: elements at or beyond `left` read as `fill` and are not written.
+// The same with the end of the row in sight: elements at or beyond `left` read as `fill` and are not written.  The loads of a
+// last partial vector are all on their way before the first is waited for.
 template <typename T>
 __device__ __forceinline__ void load8(Raw8<T> &r, const T *p, long left, float fill) {
   if (left >= 8) { r.load(p); return; }
+  r.fill(fill);
+  if (left <= 0) return;
+  T q[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r.set(i, i < left ? (float)p[i] : fill);
+  for (int i = 0; i < 7; ++i) q[i] = p[min((long)i, left - 1)];
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) y[i] = i < left ? (float)q[i] : fill;
+  y[7] = fill;
+  r.set8(y);
 }
 template <typename T>
 __device__ __forceinline__ void store8(const Raw8<T> &r, T *p, long left) {

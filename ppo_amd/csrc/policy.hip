@@ -234,28 +234,107 @@ __device__ __forceinline__ float max8(float m, const Raw8<T> &r) {
   for (int i = 0; i < 8; ++i) m = __builtin_elementwise_maximum(m, r.get(i));
   return m;
 }
+__device__ __forceinline__ void add_term(Softmax &w, float l) {
+  const float x = finite_power(l, w.m), e = exp2_fast(x);
+  w.s += e;
+  w.t = __builtin_fmaf(e, x, w.t);
+}
 template <typename T>
-__device__ __forceinline__ void sums8(float m, const Raw8<T> &r, float &s, float &t) {
+__device__ __forceinline__ void sums8(Softmax &w, const Raw8<T> &r) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = finite_power(r.get(i), m), e = exp2_fast(x);
-    s += e;
-    t = __builtin_fmaf(e, x, t);
+  for (int i = 0; i < 8; ++i) add_term(w, r.fresh(i));
+}
+
+// What an element costs in the vector unit is what bounds rows of 16-bit logits, so rows that allow it take a shorter way: with
+// the reference m of moderate size and every logit finite, x = l log2(e) - m2 is one fma against m2 = fl(m log2(e)) and needs no
+// clamp.  (m2's rounding shifts all x by `shift`, which is known exactly and taken out afterwards; its size grows with |m|.)
+constexpr float kPlainMost = 4096.f, kPlainLeast = -1e30f;
+
+struct Plain {
+  float m2, shift;       // x of the row's definition = x here - shift
+  __device__ __forceinline__ explicit Plain(float m) {
+    m2 = m * kLog2e;
+    shift = __builtin_fmaf(m, kLog2e, -m2);
+  }
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c)); return d; }
+__device__ __forceinline__ float min3(float a, float b, float c) { float d; asm("v_minimum3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c)); return d; }
+
+// What the place beyond a row's end holds: so small that its power is 0, finite so that the row's last wave need not go the long
+// way.  Where the row itself is as small, row_softmax reads its own elements once more instead.
+template <typename T> constexpr float kBeyond = -9e29f;
+template <> constexpr float kBeyond<_Float16> = -65504.f;
+
+// A row over `lanes` lanes: lane i holds vectors i, i + lanes, ...  All of them are on their way before anything waits (which is
+// why the row's end is one straight block with clamped addresses: another merge of values would make the compiler wait for each).
+template <int NV, typename T>
+__device__ __forceinline__ void load_row(Raw8<T> *r, const T *in, unsigned lane, unsigned lanes, unsigned vocab) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const unsigned e = (k * lanes + lane) * 8;
+    if (e + 8 <= vocab) {
+      r[k].load(in + e);
+    } else {
+      T q[8];
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = in[min(e + i, vocab - 1)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = e + i < vocab ? (float)q[i] : kBeyond<T>;
+      r[k].set8(y);
+    }
   }
 }
 
-// Vectors that sit in registers.
+// NV vectors in registers, `step` elements apart from element e0 on.  Returns whether the whole wave went the short way, which
+// its gradient may then go as well.
 template <int NV, typename T>
-__device__ __forceinline__ void row_softmax(Softmax &w, Raw8<T> *r) {
-#pragma unroll
-  for (int k = 0; k < NV; ++k) w.m = max8(w.m, r[k]);
-  if (w.m == -__builtin_inff()) return;                       // -inf throughout: no terms
+__device__ __forceinline__ bool row_softmax(Softmax &w, const Raw8<T> *r, const T *in, unsigned e0, unsigned step, unsigned vocab) {
+  float least = 0.f;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    r[k].pin();
-    sums8(w.m, r[k], w.s, w.t);
-    r[k].pin();
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float a = r[k].get(i), b = r[k].get(i + 1);
+      w.m = max3(w.m, a, b);
+      least = min3(least, a, b);
+    }
   }
+  if (__all(least >= kPlainLeast && __builtin_fabsf(w.m) <= kPlainMost)) {
+    const Plain p(w.m);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = __builtin_fmaf(r[k].fresh(i), kLog2e, -p.m2), e = exp2_fast(x);
+        w.s += e;
+        w.t = __builtin_fmaf(e, x, w.t);
+      }
+    }
+    const float f = exp2_fast(-p.shift);
+    w.t = (w.t - p.shift * w.s) * f;
+    w.s *= f;
+    return true;
+  }
+  if (w.m <= kBeyond<T> / 2) {                                // the row's own logits are as small as what lies beyond it, or -inf
+    w.m = -__builtin_inff();
+#pragma unroll 1
+    for (unsigned j = 0; j < NV * 8; ++j) {
+      const unsigned e = e0 + j / 8 * step + j % 8;
+      if (e < vocab) w.m = __builtin_elementwise_maximum(w.m, (float)in[e]);
+    }
+    if (w.m == -__builtin_inff()) return false;
+#pragma unroll 1
+    for (unsigned j = 0; j < NV * 8; ++j) {
+      const unsigned e = e0 + j / 8 * step + j % 8;
+      if (e < vocab) add_term(w, (float)in[e]);
+    }
+    return false;
+  }
+#pragma unroll
+  for (int k = 0; k < NV; ++k) sums8(w, r[k]);
+  return false;
 }
 
 // One pass with a running maximum.
@@ -265,7 +344,7 @@ __device__ __forceinline__ void online(Softmax &w, const Raw8<T> &r) {
   if (!(top > w.m) && w.s == 0.f) { w.m = top; return; }     // nothing but -inf so far, or NaN
   rebase(w.m, top, w.s, w.t);
   w.m = top;
-  sums8(top, r, w.s, w.t);
+  sums8(w, r);
 }
 
 // Gradient of one row's logits r (in place): dl_j = (g (p_j - 1{j = a}) + ent p_j (ln p_j + H)) / n with p_j = e_j / s and
@@ -286,12 +365,22 @@ __device__ __forceinline__ GradTerms grad_terms(const PolicyArgs &a, float m, co
   return k;
 }
 
-template <typename T>
+// ... as the short way has it: k.m holds m2.
+__device__ __forceinline__ GradTerms plain_terms(GradTerms k) {
+  const Plain p(k.m);
+  const float f = exp2_fast(-p.shift);
+  k.c0 = (k.c0 - k.c1 * p.shift) * f;
+  k.c1 *= f;
+  k.m = p.m2;
+  return k;
+}
+
+template <bool PLAIN, typename T>
 __device__ __forceinline__ void gradient8(Raw8<T> &r, const GradTerms &k, int at) {   // at: the action's place in r, if 0..7
   float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float x = finite_power(r.get(i), k.m);
+    const float l = r.fresh(i), x = PLAIN ? __builtin_fmaf(l, kLog2e, -k.m) : finite_power(l, k.m);
     y[i] = exp2_fast(x) * __builtin_fmaf(x, k.c1, k.c0);
   }
   if ((unsigned)at < 8u) {
@@ -299,11 +388,31 @@ __device__ __forceinline__ void gradient8(Raw8<T> &r, const GradTerms &k, int at
     for (int i = 0; i < 8; ++i)
       if (i == at) y[i] -= k.hit;
   }
-  if (k.nan || k.zero) {
+  if (!PLAIN && (k.nan || k.zero)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = k.zero ? 0.f : __builtin_nanf("");
   }
   r.set8(y);
+}
+
+// The gradient of a row that load_row brought, written.
+template <bool PLAIN, int NV, typename T>
+__device__ __forceinline__ void write_gradient(Raw8<T> *r, const GradTerms &k, T *out, unsigned lane, unsigned lanes, unsigned vocab,
+                                               int64_t action) {
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const unsigned e = (v * lanes + lane) * 8;
+    if (e >= vocab) break;
+    gradient8<PLAIN>(r[v], k, (int)(action - e));
+    store8(r[v], out + e, (long)(vocab - e));
+  }
+}
+// The short way only where every lane's row allows it and has a distribution.
+template <int NV, typename T>
+__device__ __forceinline__ void write_gradient(Raw8<T> *r, const GradTerms &k, T *out, unsigned lane, unsigned lanes, unsigned vocab,
+                                               int64_t action, bool plain) {
+  if (plain && __all(__builtin_fabsf(k.m) <= kPlainMost && !k.nan && !k.zero)) write_gradient<true, NV>(r, plain_terms(k), out, lane, lanes, vocab, action);
+  else write_gradient<false, NV>(r, k, out, lane, lanes, vocab, action);
 }
 
 // Up to kGroupVocab tokens: `lanes` neighbouring lanes of a wave hold one row in registers (8 elements and NV vectors each), so a
@@ -325,24 +434,22 @@ __global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigne
     RowInputs q{};
     if (LOSS && live) q = row_inputs(a, row);
     Raw8<T> r[NV];
-    float m = -__builtin_inff();
     if (action != -1) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) load8(r[k], in + (k * 64 + sub) * 8, (long)a.vocab - (k * 64 + sub) * 8, -__builtin_inff());
+      load_row<NV>(r, in, sub, lanes, a.vocab);
     } else {
 #pragma unroll
       for (int k = 0; k < NV; ++k) r[k].fill(-__builtin_inff());
     }
     const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) m = max8(m, r[k]);
+    Softmax w{-__builtin_inff(), 0.f, 0.f};
+    const bool plain = row_softmax<NV>(w, r, in, sub * 8, 512, a.vocab);
+    float m = w.m;
     for (unsigned off = 1; off < lanes; off <<= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, (int)off, 64));
-    float s = 0.f, t = 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) sums8(m, r[k], s, t);
-    for (unsigned off = 1; off < lanes; off <<= 1) { s += __shfl_xor(s, (int)off, 64); t += __shfl_xor(t, (int)off, 64); }
+    rebase(w.m, m, w.s, w.t);
+    w.m = m;
+    for (unsigned off = 1; off < lanes; off <<= 1) { w.s += __shfl_xor(w.s, (int)off, 64); w.t += __shfl_xor(w.t, (int)off, 64); }
     if (!live) continue;
-    const RowTerms o = row_terms(Softmax{m, s, t}, action, a.vocab, l_a);
+    const RowTerms o = row_terms(w, action, a.vocab, l_a);
     if (sub == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
     if (!LOSS) continue;
     const RowShare share = row_objective(a, q, o);
@@ -350,15 +457,8 @@ __global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigne
       a.dvalues[row] = share.dvalue;
       for (int i = 0; i < 5; ++i) sum[i] += share.part[i];
     }
-    const GradTerms k = grad_terms(a, m, o, share.g);
-    T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const unsigned e = (v * 64 + sub) * 8;
-      if (e >= a.vocab) break;
-      gradient8(r[v], k, (int)(action - e));
-      store8(r[v], out + e, (long)(a.vocab - e));
-    }
+    const GradTerms k = grad_terms(a, w.m, o, share.g);
+    write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride, sub, lanes, a.vocab, action, plain);
   }
   if (!LOSS) return;
   for (int i = 0; i < 5; ++i) {
@@ -402,25 +502,18 @@ __global__ __launch_bounds__(1024, NV * sizeof(Raw8<T>) <= 128 ? 8 : 4) void pol
   const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
   const RowInputs q = row_inputs(a, row);
   Raw8<T> r[NV];
+  bool plain = false;
   Softmax w{-__builtin_inff(), 0.f, 0.f};
   if (action != -1) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) load8(r[k], in + (k * threads + tid) * 8, (long)a.vocab - (k * threads + tid) * 8, -__builtin_inff());
-    row_softmax<NV>(w, r);
+    load_row<NV>(r, in, tid, threads, a.vocab);
+    plain = row_softmax<NV>(w, r, in, tid * 8, threads * 8, a.vocab);
   }
   w = block_softmax(w, red);
   const RowTerms o = row_terms(w, action, a.vocab, l_a);
   const RowShare share = row_objective(a, q, o);
   if (tid == 0) put_row(a, row, o, share);
   const GradTerms k = grad_terms(a, w.m, o, share.g);
-  T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const unsigned e = (v * threads + tid) * 8;
-    if (e >= a.vocab) break;
-    gradient8(r[v], k, (int)(action - e));
-    store8(r[v], out + e, (long)(a.vocab - e));
-  }
+  write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride, tid, threads, a.vocab, action, plain);
 }
 
 // Rows too long for the registers of a workgroup: read a second time for the gradient, out of the caches as far as they hold it.
@@ -449,7 +542,7 @@ __global__ __launch_bounds__(1024) void policy_loss_long_kernel(PolicyArgs a) {
   for (unsigned e = tid * 8; e < a.vocab; e += 8192) {
     Raw8<T> r;
     load8(r, in + e, (long)(a.vocab - e), -__builtin_inff());
-    gradient8(r, k, (int)(action - e));
+    gradient8<false>(r, k, (int)(action - e));
     store8(r, out + e, (long)(a.vocab - e));
   }
 }
@@ -467,12 +560,9 @@ __global__ __launch_bounds__(256) void policy_split_kernel(PolicyArgs a, unsigne
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
   Raw8<T> r[kSplitVecs];
   Softmax w{-__builtin_inff(), 0.f, 0.f};
-#pragma unroll
-  for (int k = 0; k < kSplitVecs; ++k) {
-    const unsigned e = c0 + (k * 256 + threadIdx.x) * 8;
-    load8(r[k], in + e, (long)a.vocab - (long)e, -__builtin_inff());
-  }
-  row_softmax<kSplitVecs>(w, r);
+  const unsigned len = min(a.vocab - c0, kSplitChunk);
+  load_row<kSplitVecs>(r, in + c0, threadIdx.x, 256, len);
+  row_softmax<kSplitVecs>(w, r, in + c0, threadIdx.x * 8, 2048, len);
   w = block_softmax(w, red);
   if (threadIdx.x == 0) {
     parts[blockIdx.x] = w;
@@ -507,11 +597,8 @@ __global__ __launch_bounds__(256) void policy_split_loss_kernel(PolicyArgs a, un
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
   T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
   Raw8<T> r[kSplitVecs];
-#pragma unroll
-  for (int k = 0; k < kSplitVecs; ++k) {
-    const unsigned e = c0 + (k * 256 + tid) * 8;
-    load8(r[k], in + e, (long)a.vocab - (long)e, -__builtin_inff());
-  }
+  const unsigned len = min(a.vocab - c0, kSplitChunk);
+  load_row<kSplitVecs>(r, in + c0, tid, 256, len);
   const RowInputs q = row_inputs(a, row);
   const int64_t action = a.actions[row];
   const Softmax w = join_chunks(parts + row * chunks, chunks);
@@ -519,13 +606,7 @@ __global__ __launch_bounds__(256) void policy_split_loss_kernel(PolicyArgs a, un
   const RowShare share = row_objective(a, q, o);
   if (chunk == 0 && tid == 0) put_row(a, row, o, share);
   const GradTerms k = grad_terms(a, w.m, o, share.g);
-#pragma unroll
-  for (int v = 0; v < kSplitVecs; ++v) {
-    const unsigned e = c0 + (v * 256 + tid) * 8;
-    if (e >= a.vocab) break;
-    gradient8(r[v], k, (int)(action - e));
-    store8(r[v], out + e, (long)(a.vocab - e));
-  }
+  write_gradient<false, kSplitVecs>(r, k, out + c0, tid, 256, len, action - c0);
 }
 
 // Sums the records in a fixed order, in 64 bits: each workgroup a slice, three waves a column; the last workgroup to finish adds
@@ -698,7 +779,7 @@ void launch_stats(const Plan &p, const PolicyArgs &a, Softmax *parts, float *pic
 }
 
 // Vectors a thread: the choice that keeps most rows in a CU at once, whose phases then overlap; of equal ones the smallest.
-// `kWaves`: waves a CU holds of the kernel with that many vectors (its registers: 24 and 4 a vector, 8 of floats).
+// `kWaves`: waves a CU holds of the kernel with that many vectors (its registers: 22 and 4 a vector, 8 of floats).
 constexpr int row_waves(int regs) { return 512 / ((regs + 7) / 8 * 8) >= 8 ? 32 : 512 / ((regs + 7) / 8 * 8) * 4; }
 
 template <typename T, int NV>
@@ -715,7 +796,7 @@ void launch_row(const PolicyArgs &a, hipStream_t s) {
   int best = 0, rows = 0;
   for (int c : choices) {
     const unsigned waves = (vecs + c / kScale * 64 - 1) / (c / kScale * 64);
-    const int held = waves <= 16 ? row_waves(28 + 4 * c) / (int)waves : 0;
+    const int held = waves <= 16 ? row_waves(22 + 4 * c) / (int)waves : 0;
     if (held > rows) { rows = held; best = c; }
   }
   switch (best) {
