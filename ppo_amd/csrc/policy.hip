@@ -266,22 +266,33 @@ __device__ __forceinline__ float min3(float a, float b, float c) { float d; asm(
 template <typename T> constexpr float kBeyond = -9e29f;
 template <> constexpr float kBeyond<_Float16> = -65504.f;
 
+// Elements first .. end of an array: a row, seen from the last 4-byte boundary at or before its start.  Sixteen bytes at a multiple of
+// two bytes only cost the row kernels 15 % (50 001 against 50 000 bf16 tokens); at a multiple of four they are free.
+struct Span { unsigned first, end; };
+
+template <typename T>
+__device__ __forceinline__ Span span_of(const T *&in, unsigned vocab) {
+  const unsigned odd = sizeof(T) == 2 ? (unsigned)((uintptr_t)in >> 1) & 1u : 0u;
+  in -= odd;
+  return Span{odd, vocab + odd};
+}
+
 // A row over `lanes` lanes: lane i holds vectors i, i + lanes, ...  All of them are on their way before anything waits (which is
-// why the row's end is one straight block with clamped addresses: another merge of values would make the compiler wait for each).
+// why the row's ends are one straight block with clamped addresses: another merge of values would make the compiler wait for each).
 template <int NV, typename T>
-__device__ __forceinline__ void load_row(Raw8<T> *r, const T *in, unsigned lane, unsigned lanes, unsigned vocab) {
+__device__ __forceinline__ void load_row(Raw8<T> *r, const T *in, unsigned lane, unsigned lanes, Span at) {
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const unsigned e = (k * lanes + lane) * 8;
-    if (e + 8 <= vocab) {
+    if (e >= at.first && e + 8 <= at.end) {
       r[k].load(in + e);
     } else {
       T q[8];
       float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = in[min(e + i, vocab - 1)];
+      for (int i = 0; i < 8; ++i) q[i] = in[max(min(e + i, at.end - 1), at.first)];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = e + i < vocab ? (float)q[i] : kBeyond<T>;
+      for (int i = 0; i < 8; ++i) y[i] = e + i >= at.first && e + i < at.end ? (float)q[i] : kBeyond<T>;
       r[k].set8(y);
     }
   }
@@ -290,7 +301,7 @@ __device__ __forceinline__ void load_row(Raw8<T> *r, const T *in, unsigned lane,
 // NV vectors in registers, `step` elements apart from element e0 on.  Returns whether the whole wave went the short way, which
 // its gradient may then go as well.
 template <int NV, typename T>
-__device__ __forceinline__ bool row_softmax(Softmax &w, const Raw8<T> *r, const T *in, unsigned e0, unsigned step, unsigned vocab) {
+__device__ __forceinline__ bool row_softmax(Softmax &w, const Raw8<T> *r, const T *in, unsigned e0, unsigned step, Span at) {
   float least = 0.f;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -322,13 +333,13 @@ __device__ __forceinline__ bool row_softmax(Softmax &w, const Raw8<T> *r, const 
 #pragma unroll 1
     for (unsigned j = 0; j < NV * 8; ++j) {
       const unsigned e = e0 + j / 8 * step + j % 8;
-      if (e < vocab) w.m = __builtin_elementwise_maximum(w.m, (float)in[e]);
+      if (e >= at.first && e < at.end) w.m = __builtin_elementwise_maximum(w.m, (float)in[e]);
     }
     if (w.m == -__builtin_inff()) return false;
 #pragma unroll 1
     for (unsigned j = 0; j < NV * 8; ++j) {
       const unsigned e = e0 + j / 8 * step + j % 8;
-      if (e < vocab) add_term(w, (float)in[e]);
+      if (e >= at.first && e < at.end) add_term(w, (float)in[e]);
     }
     return false;
   }
@@ -397,22 +408,23 @@ __device__ __forceinline__ void gradient8(Raw8<T> &r, const GradTerms &k, int at
 
 // The gradient of a row that load_row brought, written.
 template <bool PLAIN, int NV, typename T>
-__device__ __forceinline__ void write_gradient(Raw8<T> *r, const GradTerms &k, T *out, unsigned lane, unsigned lanes, unsigned vocab,
-                                               int64_t action) {
+__device__ __forceinline__ void write_gradient(Raw8<T> *r, const GradTerms &k, T *out, unsigned lane, unsigned lanes, Span at, int64_t action) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const unsigned e = (v * lanes + lane) * 8;
-    if (e >= vocab) break;
+    if (e >= at.end) break;
     gradient8<PLAIN>(r[v], k, (int)(action - e));
-    store8(r[v], out + e, (long)(vocab - e));
+    if (e >= at.first && e + 8 <= at.end) r[v].store(out + e);
+    else
+      for (int i = 0; i < 8; ++i)
+        if (e + i >= at.first && e + i < at.end) out[e + i] = (T)r[v].get(i);
   }
 }
 // The short way only where every lane's row allows it and has a distribution.
 template <int NV, typename T>
-__device__ __forceinline__ void write_gradient(Raw8<T> *r, const GradTerms &k, T *out, unsigned lane, unsigned lanes, unsigned vocab,
-                                               int64_t action, bool plain) {
-  if (plain && __all(__builtin_fabsf(k.m) <= kPlainMost && !k.nan && !k.zero)) write_gradient<true, NV>(r, plain_terms(k), out, lane, lanes, vocab, action);
-  else write_gradient<false, NV>(r, k, out, lane, lanes, vocab, action);
+__device__ __forceinline__ void write_gradient(Raw8<T> *r, const GradTerms &k, T *out, unsigned lane, unsigned lanes, Span at, int64_t action, bool plain) {
+  if (plain && __all(__builtin_fabsf(k.m) <= kPlainMost && !k.nan && !k.zero)) write_gradient<true, NV>(r, plain_terms(k), out, lane, lanes, at, action);
+  else write_gradient<false, NV>(r, k, out, lane, lanes, at, action);
 }
 
 // Up to kGroupVocab tokens: `lanes` neighbouring lanes of a wave hold one row in registers (8 elements and NV vectors each), so a
@@ -435,14 +447,14 @@ __global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigne
     if (LOSS && live) q = row_inputs(a, row);
     Raw8<T> r[NV];
     if (action != -1) {
-      load_row<NV>(r, in, sub, lanes, a.vocab);
+      load_row<NV>(r, in, sub, lanes, Span{0, a.vocab});
     } else {
 #pragma unroll
       for (int k = 0; k < NV; ++k) r[k].fill(-__builtin_inff());
     }
     const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
     Softmax w{-__builtin_inff(), 0.f, 0.f};
-    const bool plain = row_softmax<NV>(w, r, in, sub * 8, 512, a.vocab);
+    const bool plain = row_softmax<NV>(w, r, in, sub * 8, 512, Span{0, a.vocab});
     float m = w.m;
     for (unsigned off = 1; off < lanes; off <<= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, (int)off, 64));
     rebase(w.m, m, w.s, w.t);
@@ -458,7 +470,7 @@ __global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigne
       for (int i = 0; i < 5; ++i) sum[i] += share.part[i];
     }
     const GradTerms k = grad_terms(a, w.m, o, share.g);
-    write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride, sub, lanes, a.vocab, action, plain);
+    write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride, sub, lanes, Span{0, a.vocab}, action, plain);
   }
   if (!LOSS) return;
   for (int i = 0; i < 5; ++i) {
@@ -470,7 +482,9 @@ __global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigne
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
 }
 
-// One workgroup per row, statistics only: the row streams through registers once.
+// One workgroup per row, statistics only: the row streams through registers once, kStatsVecs vectors a thread at a time.
+constexpr int kStatsVecs = 4;
+
 template <typename T>
 __global__ __launch_bounds__(256) void policy_stats_row_kernel(PolicyArgs a) {
   __shared__ Softmax red[16];
@@ -478,12 +492,19 @@ __global__ __launch_bounds__(256) void policy_stats_row_kernel(PolicyArgs a) {
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
   const int64_t action = a.actions[row];
   const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
+  const Span at = span_of(in, a.vocab);
   Softmax w{-__builtin_inff(), 0.f, 0.f};
   if (action != -1)
-    for (unsigned e = threadIdx.x * 8; e < a.vocab; e += 2048) {
-      Raw8<T> r;
-      load8(r, in + e, (long)(a.vocab - e), -__builtin_inff());
-      online(w, r);
+    for (unsigned e0 = 0; e0 < at.end; e0 += kStatsVecs * 2048) {
+      Raw8<T> r[kStatsVecs];
+      const Span part{e0 ? 0u : at.first, min(at.end - e0, kStatsVecs * 2048u)};
+      load_row<kStatsVecs>(r, in + e0, threadIdx.x, 256, part);
+      Softmax q{-__builtin_inff(), 0.f, 0.f};
+      row_softmax<kStatsVecs>(q, r, in + e0, threadIdx.x * 8, 2048, part);
+      const float m = __builtin_elementwise_maximum(w.m, q.m);
+      rebase(w.m, m, w.s, w.t);
+      rebase(q.m, m, q.s, q.t);
+      w = Softmax{m, w.s + q.s, w.t + q.t};
     }
   w = block_softmax(w, red);
   const RowTerms o = row_terms(w, action, a.vocab, l_a);
@@ -501,19 +522,20 @@ __global__ __launch_bounds__(1024, NV * sizeof(Raw8<T>) <= 128 ? 8 : 4) void pol
   const int64_t action = a.actions[row];
   const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
   const RowInputs q = row_inputs(a, row);
+  const Span at = span_of(in, a.vocab);
   Raw8<T> r[NV];
   bool plain = false;
   Softmax w{-__builtin_inff(), 0.f, 0.f};
   if (action != -1) {
-    load_row<NV>(r, in, tid, threads, a.vocab);
-    plain = row_softmax<NV>(w, r, in, tid * 8, threads * 8, a.vocab);
+    load_row<NV>(r, in, tid, threads, at);
+    plain = row_softmax<NV>(w, r, in, tid * 8, threads * 8, at);
   }
   w = block_softmax(w, red);
   const RowTerms o = row_terms(w, action, a.vocab, l_a);
   const RowShare share = row_objective(a, q, o);
   if (tid == 0) put_row(a, row, o, share);
   const GradTerms k = grad_terms(a, w.m, o, share.g);
-  write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride, tid, threads, a.vocab, action, plain);
+  write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride - at.first, tid, threads, at, action + at.first, plain);
 }
 
 // Rows too long for the registers of a workgroup: read a second time for the gradient, out of the caches as far as they hold it.
@@ -561,8 +583,8 @@ __global__ __launch_bounds__(256) void policy_split_kernel(PolicyArgs a, unsigne
   Raw8<T> r[kSplitVecs];
   Softmax w{-__builtin_inff(), 0.f, 0.f};
   const unsigned len = min(a.vocab - c0, kSplitChunk);
-  load_row<kSplitVecs>(r, in + c0, threadIdx.x, 256, len);
-  row_softmax<kSplitVecs>(w, r, in + c0, threadIdx.x * 8, 2048, len);
+  load_row<kSplitVecs>(r, in + c0, threadIdx.x, 256, Span{0, len});
+  row_softmax<kSplitVecs>(w, r, in + c0, threadIdx.x * 8, 2048, Span{0, len});
   w = block_softmax(w, red);
   if (threadIdx.x == 0) {
     parts[blockIdx.x] = w;
@@ -598,7 +620,7 @@ __global__ __launch_bounds__(256) void policy_split_loss_kernel(PolicyArgs a, un
   T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
   Raw8<T> r[kSplitVecs];
   const unsigned len = min(a.vocab - c0, kSplitChunk);
-  load_row<kSplitVecs>(r, in + c0, tid, 256, len);
+  load_row<kSplitVecs>(r, in + c0, tid, 256, Span{0, len});
   const RowInputs q = row_inputs(a, row);
   const int64_t action = a.actions[row];
   const Softmax w = join_chunks(parts + row * chunks, chunks);
@@ -606,7 +628,7 @@ __global__ __launch_bounds__(256) void policy_split_loss_kernel(PolicyArgs a, un
   const RowShare share = row_objective(a, q, o);
   if (chunk == 0 && tid == 0) put_row(a, row, o, share);
   const GradTerms k = grad_terms(a, w.m, o, share.g);
-  write_gradient<false, kSplitVecs>(r, k, out + c0, tid, 256, len, action - c0);
+  write_gradient<false, kSplitVecs>(r, k, out + c0, tid, 256, Span{0, len}, action - c0);
 }
 
 // Sums the records in a fixed order, in 64 bits: each workgroup a slice, three waves a column; the last workgroup to finish adds
@@ -720,7 +742,7 @@ int shape(const char *who, int device, void *stream, int dtype, ShapeArgs &a, si
 }
 
 // Which kernels a call takes, and what they need.
-enum Route { kGroup, kRow, kLong, kSplit };
+enum Route { kGroup, kRow, kSplit };
 
 struct Plan {
   Route route;
@@ -732,7 +754,6 @@ struct Plan {
 
 // Few rows leave most of the 256 CUs idle with one workgroup each; the split costs a launch and a second read out of the caches.
 constexpr size_t kSplitRows = 256, kSplitVocab = 2 * kSplitChunk;
-constexpr size_t kRowBytes = size_t(1024) * 16 * 16;      // what 1024 threads hold in 16 vectors of 16 bytes
 
 Plan plan_of(int dtype, size_t rows, size_t vocab, bool loss) {
   Plan p;
@@ -746,7 +767,7 @@ Plan plan_of(int dtype, size_t rows, size_t vocab, bool loss) {
     p.route = kSplit;
     p.chunks = (unsigned)((vocab + kSplitChunk - 1) / kSplitChunk);
   } else {
-    p.route = !loss || vocab * dtype_bytes(dtype) <= kRowBytes ? kRow : kLong;
+    p.route = kRow;
   }
   p.records = p.route == kGroup ? p.blocks : rows;
   if (loss) p.bytes = p.records * 5 * sizeof(double);
@@ -792,7 +813,8 @@ template <typename T>
 void launch_row(const PolicyArgs &a, hipStream_t s) {
   constexpr int kScale = sizeof(T) / 2;                 // 16-byte registers of 8 elements
   static const int choices[] = {4, 6, 8, 10, 12, 14, 16};
-  const unsigned vecs = (a.vocab + 7) / 8;
+  const bool odd = (uintptr_t)a.logits % 4 || (a.rows > 1 && a.stride * sizeof(T) % 4);   // some row starts with half a word
+  const unsigned vecs = (a.vocab + odd + 7) / 8;
   int best = 0, rows = 0;
   for (int c : choices) {
     const unsigned waves = (vecs + c / kScale * 64 - 1) / (c / kScale * 64);
@@ -806,7 +828,8 @@ void launch_row(const PolicyArgs &a, hipStream_t s) {
     case 10: launch_row_as<T, 10 / kScale>(a, vecs, s); break;
     case 12: launch_row_as<T, 12 / kScale>(a, vecs, s); break;
     case 14: launch_row_as<T, 14 / kScale>(a, vecs, s); break;
-    default: launch_row_as<T, 16 / kScale>(a, vecs, s); break;
+    case 16: launch_row_as<T, 16 / kScale>(a, vecs, s); break;
+    default: hipLaunchKernelGGL(policy_loss_long_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, s, a); break;
   }
 }
 
@@ -817,8 +840,7 @@ void launch_loss(const Plan &p, const PolicyArgs &a, Softmax *parts, float *pick
   else if (p.route == kSplit) {
     hipLaunchKernelGGL(policy_split_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, parts, picked);
     hipLaunchKernelGGL(policy_split_loss_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, (const Softmax *)parts, (const float *)picked);
-  } else if (p.route == kLong) hipLaunchKernelGGL(policy_loss_long_kernel<T>, dim3(rows), dim3(1024), 0, s, a);
-  else launch_row<T>(a, s);
+  } else launch_row<T>(a, s);
 }
 
 int check_workspace(const char *who, const Plan &p, const void *ws, size_t bytes) {
