@@ -126,6 +126,23 @@ __device__ __forceinline__ float wave_sum(float x) {
   x += dpp<0x143, 0xc>(0.f, x);
   return last_lane(x);
 }
+// Over `lanes` (a power of two) neighbouring lanes, the same in each of them: inside 16 lanes by permutations of the vector unit.
+template <typename Op>
+__device__ __forceinline__ float group_reduce(float x, unsigned lanes, Op op) {
+  if (lanes > 1) x = op(x, dpp<0xb1, 0xf>(x, x));      // the other lane of a pair
+  if (lanes > 2) x = op(x, dpp<0x4e, 0xf>(x, x));      // the other pair of four
+  if (lanes > 4) x = op(x, dpp<0x141, 0xf>(x, x));     // mirrored within eight
+  if (lanes > 8) x = op(x, dpp<0x140, 0xf>(x, x));     // mirrored within sixteen
+  if (lanes > 16) x = op(x, __shfl_xor(x, 16, 64));
+  if (lanes > 32) x = op(x, __shfl_xor(x, 32, 64));
+  return x;
+}
+__device__ __forceinline__ float group_max_nan(float x, unsigned lanes) {
+  return group_reduce(x, lanes, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+}
+__device__ __forceinline__ float group_sum(float x, unsigned lanes) {
+  return group_reduce(x, lanes, [](float a, float b) { return a + b; });
+}
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);

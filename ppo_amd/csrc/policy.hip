@@ -427,41 +427,58 @@ __device__ __forceinline__ void write_gradient(Raw8<T> *r, const GradTerms &k, T
   else write_gradient<false, NV>(r, k, out, lane, lanes, at, action);
 }
 
-// Up to kGroupVocab tokens: `lanes` neighbouring lanes of a wave hold one row in registers (8 elements and NV vectors each), so a
-// wave works on 64 / lanes rows and nothing passes through LDS.  Workgroups walk over the rows, which keeps the partial sums of
-// the objective few: one record a workgroup, added up in row order.
-constexpr unsigned kGroupVocab = 2048, kGroupBlocks = 2048;
+// One record of the objective a workgroup that walks over several rows, its waves' sums added in order.
+__device__ __forceinline__ void put_block(const PolicyArgs &a, const double sum[5], double (*red)[5]) {
+  for (int i = 0; i < 5; ++i) {
+    const double x = wave_sum(sum[i]);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64][i] = x;
+  }
+  __syncthreads();
+  if (threadIdx.x < 5) a.partials[threadIdx.x * (size_t)gridDim.x + blockIdx.x] = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
+}
 
-template <typename T, bool LOSS, int NV>
-__global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigned lanes_log2) {
+// Up to kSmallVocab tokens, the action sets of ordinary environments among them: lane i of a row's `lanes` lanes holds elements
+// i, i + lanes, ... as floats (SLOTS of them), with their powers kept for the gradient.  What a row costs beside its elements is
+// as much as 10 of them, so a row gets as few lanes as 8 elements each allow.
+constexpr unsigned kSmallVocab = 512, kGroupBlocks = 1024;
+
+template <typename T, bool LOSS, int SLOTS>
+__global__ __launch_bounds__(256) void policy_small_kernel(PolicyArgs a, unsigned lanes_log2) {
   __shared__ double red[4][5];
   const unsigned lanes = 1u << lanes_log2, sub = threadIdx.x & (lanes - 1);
   const size_t per_block = 256u >> lanes_log2;
   double sum[5] = {0, 0, 0, 0, 0};
   for (size_t row0 = blockIdx.x * per_block; row0 < a.rows; row0 += gridDim.x * per_block) {
-    const size_t row = row0 + (threadIdx.x >> lanes_log2);
-    const bool live = row < a.rows;
+    const size_t place = row0 + (threadIdx.x >> lanes_log2), row = min(place, a.rows - 1);   // every lane stays, for the permutations
+    const bool live = place < a.rows;
     const T *in = (const T *)a.logits + (int64_t)row * a.stride;
-    const int64_t action = live ? a.actions[row] : -1;
-    RowInputs q{};
-    if (LOSS && live) q = row_inputs(a, row);
-    Raw8<T> r[NV];
-    if (action != -1) {
-      load_row<NV>(r, in, sub, lanes, Span{0, a.vocab});
-    } else {
+    T raw[SLOTS];
 #pragma unroll
-      for (int k = 0; k < NV; ++k) r[k].fill(-__builtin_inff());
-    }
+    for (int i = 0; i < SLOTS; ++i) raw[i] = in[min(i * lanes + sub, a.vocab - 1)];
+    const int64_t action = a.actions[row];
+    RowInputs q{};
+    if (LOSS) q = row_inputs(a, row);
     const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[action] : 0.f;
+    float x[SLOTS], e[SLOTS];
     Softmax w{-__builtin_inff(), 0.f, 0.f};
-    const bool plain = row_softmax<NV>(w, r, in, sub * 8, 512, Span{0, a.vocab});
-    float m = w.m;
-    for (unsigned off = 1; off < lanes; off <<= 1) m = __builtin_elementwise_maximum(m, __shfl_xor(m, (int)off, 64));
-    rebase(w.m, m, w.s, w.t);
-    w.m = m;
-    for (unsigned off = 1; off < lanes; off <<= 1) { w.s += __shfl_xor(w.s, (int)off, 64); w.t += __shfl_xor(w.t, (int)off, 64); }
-    if (!live) continue;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      x[i] = i * lanes + sub < a.vocab ? (float)raw[i] : -__builtin_inff();
+      w.m = __builtin_elementwise_maximum(w.m, x[i]);
+    }
+    w.m = group_max_nan(w.m, lanes);
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      x[i] = finite_power(x[i], w.m);
+      e[i] = exp2_fast(x[i]);
+      w.s += e[i];
+      w.t = __builtin_fmaf(e[i], x[i], w.t);
+    }
+    w.s = group_sum(w.s, lanes);
+    w.t = group_sum(w.t, lanes);
     const RowTerms o = row_terms(w, action, a.vocab, l_a);
+    if (!live) continue;
     if (sub == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
     if (!LOSS) continue;
     const RowShare share = row_objective(a, q, o);
@@ -470,16 +487,52 @@ __global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a, unsigne
       for (int i = 0; i < 5; ++i) sum[i] += share.part[i];
     }
     const GradTerms k = grad_terms(a, w.m, o, share.g);
-    write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride, sub, lanes, Span{0, a.vocab}, action, plain);
+    T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const unsigned at = i * lanes + sub;
+      float y = e[i] * __builtin_fmaf(x[i], k.c1, k.c0);
+      if ((int64_t)at == action) y -= k.hit;
+      if (k.nan) y = __builtin_nanf("");
+      if (k.zero) y = 0.f;
+      if (at < a.vocab) out[at] = (T)y;
+    }
   }
-  if (!LOSS) return;
-  for (int i = 0; i < 5; ++i) {
-    const double x = wave_sum(sum[i]);
-    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64][i] = x;
+  if (LOSS) put_block(a, sum, red);
+}
+
+// Up to kGroupVocab tokens: a wave's lanes hold one row, 8 elements and NV vectors each.
+constexpr unsigned kGroupVocab = 2047;
+
+template <typename T, bool LOSS, int NV>
+__global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a) {
+  __shared__ double red[4][5];
+  const unsigned lane = threadIdx.x % 64;
+  double sum[5] = {0, 0, 0, 0, 0};
+  for (size_t row = blockIdx.x * 4 + threadIdx.x / 64; row < a.rows; row += gridDim.x * 4) {
+    const T *in = (const T *)a.logits + (int64_t)row * a.stride;
+    const Span at = span_of(in, a.vocab);
+    Raw8<T> r[NV];
+    load_row<NV>(r, in, lane, 64, at);
+    const int64_t action = a.actions[row];
+    RowInputs q{};
+    if (LOSS) q = row_inputs(a, row);
+    const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[at.first + action] : 0.f;
+    Softmax w{-__builtin_inff(), 0.f, 0.f};
+    const bool plain = row_softmax<NV>(w, r, in, lane * 8, 512, at);
+    w = wave_softmax(w);
+    const RowTerms o = row_terms(w, action, a.vocab, l_a);
+    if (lane == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
+    if (!LOSS) continue;
+    const RowShare share = row_objective(a, q, o);
+    if (lane == 0) {
+      a.dvalues[row] = share.dvalue;
+      for (int i = 0; i < 5; ++i) sum[i] += share.part[i];
+    }
+    const GradTerms k = grad_terms(a, w.m, o, share.g);
+    write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride - at.first, lane, 64, at, action + at.first, plain);
   }
-  __syncthreads();
-  if (threadIdx.x < 5) a.partials[threadIdx.x * (size_t)gridDim.x + blockIdx.x] = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
+  if (LOSS) put_block(a, sum, red);
 }
 
 // One workgroup per row, statistics only: the row streams through registers once, kStatsVecs vectors a thread at a time.
@@ -742,12 +795,12 @@ int shape(const char *who, int device, void *stream, int dtype, ShapeArgs &a, si
 }
 
 // Which kernels a call takes, and what they need.
-enum Route { kGroup, kRow, kSplit };
+enum Route { kSmall, kGroup, kRow, kSplit };
 
 struct Plan {
-  Route route;
-  unsigned lanes_log2 = 0, vecs = 1, chunks = 0;   // kGroup: lanes of a row and vectors a lane; kSplit: chunks of a row
-  unsigned blocks = 0;                             // kGroup
+  Route route = kRow;
+  unsigned lanes_log2 = 0, chunks = 0;             // kSmall, kGroup: lanes of a row; kSplit: chunks of a row
+  unsigned blocks = 0;                             // kSmall, kGroup: workgroups, which walk over the rows
   size_t records = 0;                              // of the objective
   size_t o_slices = 0, o_ticket = 0, o_parts = 0, o_picked = 0, bytes = 0;
 };
@@ -758,18 +811,16 @@ constexpr size_t kSplitRows = 256, kSplitVocab = 2 * kSplitChunk;
 Plan plan_of(int dtype, size_t rows, size_t vocab, bool loss) {
   Plan p;
   if (vocab <= kGroupVocab) {
-    p.route = kGroup;
+    p.route = vocab <= kSmallVocab ? kSmall : kGroup;
+    if (p.route == kGroup) p.lanes_log2 = 6;
     while ((8u << p.lanes_log2) < vocab && p.lanes_log2 < 6) ++p.lanes_log2;
-    p.vecs = vocab <= 512 ? 1 : vocab <= 1024 ? 2 : 4;
     const size_t per = 256u >> p.lanes_log2;
-    p.blocks = (unsigned)std::min<size_t>((rows + per - 1) / per, loss ? kGroupBlocks : kMaxGrid);
+    p.blocks = (unsigned)std::min<size_t>((rows + per - 1) / per, kGroupBlocks);
   } else if (rows < kSplitRows && vocab >= kSplitVocab) {
     p.route = kSplit;
     p.chunks = (unsigned)((vocab + kSplitChunk - 1) / kSplitChunk);
-  } else {
-    p.route = kRow;
   }
-  p.records = p.route == kGroup ? p.blocks : rows;
+  p.records = p.blocks ? p.blocks : rows;
   if (loss) p.bytes = p.records * 5 * sizeof(double);
   p.o_slices = p.bytes;
   if (loss) p.bytes += kStatsBlocks * 5 * sizeof(double);
@@ -784,15 +835,26 @@ Plan plan_of(int dtype, size_t rows, size_t vocab, bool loss) {
 
 template <typename T, bool LOSS>
 void launch_group(const Plan &p, const PolicyArgs &a, hipStream_t s) {
-  if (p.vecs == 1) hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 1>), dim3(p.blocks), dim3(256), 0, s, a, p.lanes_log2);
-  else if (p.vecs == 2) hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 2>), dim3(p.blocks), dim3(256), 0, s, a, p.lanes_log2);
-  else hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 4>), dim3(p.blocks), dim3(256), 0, s, a, p.lanes_log2);
+  const dim3 grid(p.blocks), block(256);
+  if (p.route == kGroup) {
+    if (a.vocab <= 1023) hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 2>), grid, block, 0, s, a);       // an odd address adds an element in front
+    else if (a.vocab <= 1535) hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 3>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 4>), grid, block, 0, s, a);
+    return;
+  }
+  const unsigned slots = (a.vocab + (1u << p.lanes_log2) - 1) >> p.lanes_log2;
+  if (slots <= 2) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 2>), grid, block, 0, s, a, p.lanes_log2);
+  else if (slots <= 4) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 4>), grid, block, 0, s, a, p.lanes_log2);
+  else if (slots == 5) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 5>), grid, block, 0, s, a, p.lanes_log2);
+  else if (slots == 6) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 6>), grid, block, 0, s, a, p.lanes_log2);
+  else if (slots == 7) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 7>), grid, block, 0, s, a, p.lanes_log2);
+  else hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 8>), grid, block, 0, s, a, p.lanes_log2);
 }
 
 template <typename T>
 void launch_stats(const Plan &p, const PolicyArgs &a, Softmax *parts, float *picked, hipStream_t s) {
   const unsigned rows = (unsigned)a.rows;
-  if (p.route == kGroup) launch_group<T, false>(p, a, s);
+  if (p.blocks) launch_group<T, false>(p, a, s);
   else if (p.route == kSplit) {
     hipLaunchKernelGGL(policy_split_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, parts, picked);
     hipLaunchKernelGGL(policy_join_kernel, dim3(rows), dim3(64), 0, s, a, p.chunks, (const Softmax *)parts, (const float *)picked);
@@ -836,7 +898,7 @@ void launch_row(const PolicyArgs &a, hipStream_t s) {
 template <typename T>
 void launch_loss(const Plan &p, const PolicyArgs &a, Softmax *parts, float *picked, hipStream_t s) {
   const unsigned rows = (unsigned)a.rows;
-  if (p.route == kGroup) launch_group<T, true>(p, a, s);
+  if (p.blocks) launch_group<T, true>(p, a, s);
   else if (p.route == kSplit) {
     hipLaunchKernelGGL(policy_split_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, parts, picked);
     hipLaunchKernelGGL(policy_split_loss_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, (const Softmax *)parts, (const float *)picked);
