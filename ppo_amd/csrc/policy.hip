@@ -271,8 +271,8 @@ template <> constexpr float kBeyond<_Float16> = -65504.f;
 struct Span { unsigned first, end; };
 
 template <typename T>
-__device__ __forceinline__ Span span_of(const T *&in, unsigned vocab) {
-  const unsigned odd = sizeof(T) == 2 ? (unsigned)((uintptr_t)in >> 1) & 1u : 0u;
+__device__ __forceinline__ Span span_of(const T *&in, unsigned vocab, bool room = true) {   // room: for an element in front
+  const unsigned odd = sizeof(T) == 2 && room ? (unsigned)((uintptr_t)in >> 1) & 1u : 0u;
   in -= odd;
   return Span{odd, vocab + odd};
 }
@@ -438,10 +438,10 @@ __device__ __forceinline__ void put_block(const PolicyArgs &a, const double sum[
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
 }
 
-// Up to kSmallVocab tokens, the action sets of ordinary environments among them: lane i of a row's `lanes` lanes holds elements
+// Up to kSmallVocab tokens, the action sets of ordinary environments: lane i of a row's `lanes` lanes holds elements
 // i, i + lanes, ... as floats (SLOTS of them), with their powers kept for the gradient.  What a row costs beside its elements is
 // as much as 10 of them, so a row gets as few lanes as 8 elements each allow.
-constexpr unsigned kSmallVocab = 512, kGroupBlocks = 1024;
+constexpr unsigned kSmallVocab = 32, kGroupBlocks = 1024;
 
 template <typename T, bool LOSS, int SLOTS>
 __global__ __launch_bounds__(256) void policy_small_kernel(PolicyArgs a, unsigned lanes_log2) {
@@ -501,44 +501,48 @@ __global__ __launch_bounds__(256) void policy_small_kernel(PolicyArgs a, unsigne
   if (LOSS) put_block(a, sum, red);
 }
 
-// Up to kGroupVocab tokens: a wave's lanes hold one row, 8 elements and NV vectors each.
-constexpr unsigned kGroupVocab = 2047;
+// Up to kGroupVocab tokens: `lanes` neighbouring lanes hold one row, NV vectors of 8 each, and a wave as many rows as it can: what a
+// row costs beside its elements (some 200 instructions) is paid once a wave.
+constexpr unsigned kGroupVocab = 2048;
 
 template <typename T, bool LOSS, int NV>
-__global__ __launch_bounds__(256) void policy_group_kernel(PolicyArgs a) {
+__global__ __launch_bounds__(256, 4) void policy_group_kernel(PolicyArgs a, unsigned lanes_log2) {
   __shared__ double red[4][5];
-  const unsigned lane = threadIdx.x % 64;
+  const unsigned lanes = 1u << lanes_log2, sub = threadIdx.x & (lanes - 1);
+  const size_t per_block = 256u >> lanes_log2;
   double sum[5] = {0, 0, 0, 0, 0};
-  for (size_t row = blockIdx.x * 4 + threadIdx.x / 64; row < a.rows; row += gridDim.x * 4) {
+  for (size_t row0 = blockIdx.x * per_block; row0 < a.rows; row0 += gridDim.x * per_block) {
+    const size_t place = row0 + (threadIdx.x >> lanes_log2), row = min(place, a.rows - 1);   // every lane stays, for the permutations
+    const bool live = place < a.rows;
     const T *in = (const T *)a.logits + (int64_t)row * a.stride;
-    const Span at = span_of(in, a.vocab);
+    const Span at = span_of(in, a.vocab, a.vocab < NV * 8 * lanes);
     Raw8<T> r[NV];
-    load_row<NV>(r, in, lane, 64, at);
+    load_row<NV>(r, in, sub, lanes, at);
     const int64_t action = a.actions[row];
     RowInputs q{};
     if (LOSS) q = row_inputs(a, row);
     const float l_a = action >= 0 && action < (int64_t)a.vocab ? (float)in[at.first + action] : 0.f;
     Softmax w{-__builtin_inff(), 0.f, 0.f};
-    const bool plain = row_softmax<NV>(w, r, in, lane * 8, 512, at);
-    w = wave_softmax(w);
+    const bool plain = row_softmax<NV>(w, r, in, sub * 8, lanes * 8, at);
+    const float m = group_max_nan(w.m, lanes);
+    rebase(w.m, m, w.s, w.t);
+    w = Softmax{m, group_sum(w.s, lanes), group_sum(w.t, lanes)};
     const RowTerms o = row_terms(w, action, a.vocab, l_a);
-    if (lane == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
+    if (live && sub == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
     if (!LOSS) continue;
     const RowShare share = row_objective(a, q, o);
-    if (lane == 0) {
+    if (live && sub == 0) {
       a.dvalues[row] = share.dvalue;
       for (int i = 0; i < 5; ++i) sum[i] += share.part[i];
     }
     const GradTerms k = grad_terms(a, w.m, o, share.g);
-    write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride - at.first, lane, 64, at, action + at.first, plain);
+    write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride - at.first, sub, lanes, live ? at : Span{0, 0}, action + at.first, plain);
   }
   if (LOSS) put_block(a, sum, red);
 }
 
-// One workgroup per row, statistics only: the row streams through registers once, kStatsVecs vectors a thread at a time.
-constexpr int kStatsVecs = 4;
-
-template <typename T>
+// One workgroup per row, statistics only: the row streams through registers once, a few vectors a thread at a time.
+template <typename T, int kStatsVecs>
 __global__ __launch_bounds__(256) void policy_stats_row_kernel(PolicyArgs a) {
   __shared__ Softmax red[16];
   const size_t row = blockIdx.x;
@@ -812,8 +816,7 @@ Plan plan_of(int dtype, size_t rows, size_t vocab, bool loss) {
   Plan p;
   if (vocab <= kGroupVocab) {
     p.route = vocab <= kSmallVocab ? kSmall : kGroup;
-    if (p.route == kGroup) p.lanes_log2 = 6;
-    while ((8u << p.lanes_log2) < vocab && p.lanes_log2 < 6) ++p.lanes_log2;
+    while ((p.route == kSmall ? 8u : 32u) << p.lanes_log2 < vocab) ++p.lanes_log2;
     const size_t per = 256u >> p.lanes_log2;
     p.blocks = (unsigned)std::min<size_t>((rows + per - 1) / per, kGroupBlocks);
   } else if (rows < kSplitRows && vocab >= kSplitVocab) {
@@ -837,9 +840,9 @@ template <typename T, bool LOSS>
 void launch_group(const Plan &p, const PolicyArgs &a, hipStream_t s) {
   const dim3 grid(p.blocks), block(256);
   if (p.route == kGroup) {
-    if (a.vocab <= 1023) hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 2>), grid, block, 0, s, a);       // an odd address adds an element in front
-    else if (a.vocab <= 1535) hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 3>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 4>), grid, block, 0, s, a);
+    const unsigned vecs = ((a.vocab + 7) / 8 + (1u << p.lanes_log2) - 1) >> p.lanes_log2;
+    if (vecs <= 3) hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 3>), grid, block, 0, s, a, p.lanes_log2);
+    else hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 4>), grid, block, 0, s, a, p.lanes_log2);
     return;
   }
   const unsigned slots = (a.vocab + (1u << p.lanes_log2) - 1) >> p.lanes_log2;
@@ -858,7 +861,9 @@ void launch_stats(const Plan &p, const PolicyArgs &a, Softmax *parts, float *pic
   else if (p.route == kSplit) {
     hipLaunchKernelGGL(policy_split_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, parts, picked);
     hipLaunchKernelGGL(policy_join_kernel, dim3(rows), dim3(64), 0, s, a, p.chunks, (const Softmax *)parts, (const float *)picked);
-  } else hipLaunchKernelGGL(policy_stats_row_kernel<T>, dim3(rows), dim3(256), 0, s, a);
+  } else if (a.vocab < kSplitChunk) hipLaunchKernelGGL((policy_stats_row_kernel<T, 1>), dim3(rows), dim3(256), 0, s, a);
+  else if (a.vocab < 2 * kSplitChunk) hipLaunchKernelGGL((policy_stats_row_kernel<T, 2>), dim3(rows), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((policy_stats_row_kernel<T, 4>), dim3(rows), dim3(256), 0, s, a);
 }
 
 // Vectors a thread: the choice that keeps most rows in a CU at once, whose phases then overlap; of equal ones the smallest.
