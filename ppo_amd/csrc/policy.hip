@@ -20,7 +20,9 @@ struct ShapeArgs {
   const void *logits;    // backward: the logits, for the sign of tokens that were seen
   void *out;
   int64_t in_stride, logits_stride, out_stride;
-  unsigned vocab, chunks;
+  size_t rows;
+  unsigned vocab, chunks;                       // chunks of a row, where a row fills a workgroup
+  unsigned rows_per, units, magic, scan_log2;   // else rows of a workgroup, 8-element units of a row, 2^20 / units, lanes that scan a row
   ppo_xp_logit_rules r;
 };
 
@@ -28,88 +30,199 @@ constexpr int kShapeVecs = 4;                        // 8-element vectors a thre
 constexpr unsigned kShapeChunk = 256 * 8 * kShapeVecs;
 constexpr unsigned kPromptOnly = 0x80000000u;        // table word: occurrences in the generated part, this bit: in the rest
 
-// One workgroup shapes one chunk of one row's vocabulary.  With a history it counts the row's tokens that fall into its chunk
-// in LDS first (integer atomics: the order does not matter), while its logits are already on their way into registers.
-template <typename T, bool HIST, bool BACKWARD>
+// Where element e of a workgroup's chunk has its table word: the lower and the upper halves of the vectors lie apart, so that a
+// wave reads each half without bank conflicts.
+__device__ __forceinline__ unsigned table_slot(unsigned e) { return ((e & 4) ? kShapeChunk / 2 : 0) + (e >> 3) * 4 + (e & 3); }
+
+struct RowRules {
+  float rep, inv_rep, pres, freq, inv_t;
+  const float *bias;
+  const uint8_t *mask;
+};
+
+__device__ __forceinline__ RowRules row_rules(const ppo_xp_logit_rules &r, size_t row) {
+  RowRules q;
+  q.rep = r.repetition_rows ? r.repetition_rows[row] : r.repetition;
+  q.inv_rep = 1.f / q.rep;
+  q.pres = r.presence_rows ? r.presence_rows[row] : r.presence;
+  q.freq = r.frequency_rows ? r.frequency_rows[row] : r.frequency;
+  q.inv_t = 1.f / (r.temperature_rows ? r.temperature_rows[row] : r.temperature);
+  q.bias = r.bias ? r.bias + (int64_t)row * r.bias_stride : nullptr;
+  q.mask = nullptr;
+  if (r.mask_kind != PPO_XP_MASK_NONE) {
+    const int64_t m = r.mask_row ? r.mask_row[row] : (r.mask_stride == 0 ? 0 : (int64_t)row);
+    if (m >= 0 && m < r.mask_rows) q.mask = (const uint8_t *)r.mask + m * r.mask_stride * (r.mask_kind == PPO_XP_MASK_BITS ? 4 : 1);
+  }
+  return q;
+}
+
+// Bit i: element e + i of a row is allowed.
+__device__ __forceinline__ unsigned allowed8(const RowRules &q, int kind, unsigned e, unsigned vocab) {
+  if (!q.mask) return 0xffu;
+  if (kind == PPO_XP_MASK_BITS) return q.mask[e / 8];
+  unsigned ok = 0;
+  if (e + 8 <= vocab) {
+    typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
+    const u32x2 w = *(const u32x2_a1 *)(q.mask + e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ok |= ((w[i >> 2] >> (8 * (i & 3))) & 0xffu) ? 1u << i : 0u;
+  } else {
+    for (unsigned i = 0; e + i < vocab; ++i) ok |= (q.mask[e + i] ? 1u : 0u) << i;
+  }
+  return ok;
+}
+
+// One workgroup shapes one chunk of one row's vocabulary, or several whole rows (MULTI).  With a history it enters the tokens that
+// fall into its part in an LDS table first, while its logits are already on their way into registers: their counts (integer
+// atomics, the order does not matter), or in the backward pass the slope, which every occurrence knows from the token's logit.
+// Every workgroup of a row reads the row's whole history; that is cheaper than sorting it while the history is shorter than the
+// vocabulary.  Elements then take their word without a branch: at a seen token in a hundred a wave would enter it anyway.
+template <typename T, bool HIST, bool BACKWARD, bool MULTI>
 __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
   __shared__ __attribute__((aligned(16))) unsigned table[HIST ? kShapeChunk : 4];
   const ppo_xp_logit_rules &r = a.r;
-  const size_t row = blockIdx.x / a.chunks;
-  const unsigned c0 = (blockIdx.x % a.chunks) * kShapeChunk, tid = threadIdx.x;
-  const T *in = (const T *)a.in + (int64_t)row * a.in_stride;
-  T *out = (T *)a.out + (int64_t)row * a.out_stride;
+  const unsigned tid = threadIdx.x;
+  const size_t row0 = MULTI ? (size_t)blockIdx.x * a.rows_per : blockIdx.x / a.chunks;
+  const unsigned c0 = MULTI ? 0 : (blockIdx.x % a.chunks) * kShapeChunk;
+  const unsigned here = MULTI ? (unsigned)min((size_t)a.rows_per, a.rows - row0) : 1;    // rows of this workgroup
+  RowRules one;
+  if (!MULTI) one = row_rules(r, row0);
+  // unit k of this thread: its row and first element, and whether there is one
+  auto place = [&](int k, size_t &row, unsigned &e) {
+    const unsigned u = k * 256 + tid;
+    if (!MULTI) { row = row0; e = c0 + u * 8; return e < a.vocab; }
+    const unsigned rl = (u * a.magic) >> 20;
+    row = row0 + rl;
+    e = (u - rl * a.units) * 8;
+    return rl < here;
+  };
 
   Raw8<T> raw[kShapeVecs];
 #pragma unroll
   for (int k = 0; k < kShapeVecs; ++k) {
-    const unsigned e = c0 + (k * 256 + tid) * 8;
-    if (e < a.vocab) load8(raw[k], in + e, (long)(a.vocab - e), 0.f);
+    size_t row; unsigned e;
+    const bool live = place(k, row, e);
+    if (live && e + 8 <= a.vocab) {
+      raw[k].load((const T *)a.in + (int64_t)row * a.in_stride + e);
+    } else {                                         // a row's end, or nothing: clamped addresses, no further branch
+      const T *p = (const T *)a.in + (int64_t)(live ? row : row0) * a.in_stride;
+      T q[8];
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = p[min(e + i, a.vocab - 1)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = (float)q[i];
+      raw[k].set8(y);
+    }
   }
   if (HIST) {
-    for (unsigned i = tid * 4; i < kShapeChunk; i += 1024) *(u32x4 *)(table + i) = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < kShapeVecs; ++k) {
+      unsigned word = 0;
+      if (BACKWARD) {
+        float inv_t = one.inv_t;
+        if (MULTI) {
+          size_t row; unsigned e;
+          const bool live = place(k, row, e);
+          inv_t = row_rules(r, live ? row : row0).inv_t;
+        }
+        word = __builtin_bit_cast(unsigned, inv_t);
+      }
+      *(u32x4 *)(table + (k * 256 + tid) * 4) = u32x4(word);
+      *(u32x4 *)(table + kShapeChunk / 2 + (k * 256 + tid) * 4) = u32x4(word);
+    }
     __syncthreads();
-    const int64_t h = r.hist_row ? r.hist_row[row] : (int64_t)row;
-    if (h >= 0 && h < r.hist_rows) {
-      const int64_t end = r.hist_end ? min((int64_t)r.hist_end[row], r.hist_len) : r.hist_len;
-      const int64_t begin = r.hist_begin ? max((int64_t)r.hist_begin[row], (int64_t)0) : 0;
-      const int64_t gen = r.gen_begin ? (int64_t)r.gen_begin[row] : begin;
+    const unsigned lanes = MULTI ? 1u << a.scan_log2 : 256u;
+    for (unsigned rl = MULTI ? tid >> a.scan_log2 : 0; rl < here; rl += MULTI ? 256u >> a.scan_log2 : 1u) {
+      const size_t row = row0 + rl;
+      const int64_t h = r.hist_row ? r.hist_row[row] : (int64_t)row;
+      if (h < 0 || h >= r.hist_rows) continue;
+      const int end = (int)min(r.hist_end ? (int64_t)r.hist_end[row] : r.hist_len, r.hist_len);
+      const int begin = r.hist_begin ? max(r.hist_begin[row], 0) : 0;
+      const int gen = r.gen_begin ? r.gen_begin[row] : begin;
       const int64_t base = h * r.hist_row_stride;
-      for (int64_t k = begin + tid; k < end; k += 256) {
-        const int64_t at = base + k * r.hist_tok_stride;
-        const int64_t tok = r.history_bits == 64 ? ((const int64_t *)r.history)[at] : (int64_t)((const int32_t *)r.history)[at];
-        const int64_t slot = tok - c0;
-        if (slot < 0 || slot >= kShapeChunk || tok >= a.vocab) continue;
-        if (k >= gen) atomicAdd(&table[slot], 1u);
-        else atomicOr(&table[slot], kPromptOnly);
+      const T *logits = BACKWARD ? (const T *)a.logits + (int64_t)row * a.logits_stride : nullptr;
+      float up = 0.f, down = 0.f;                    // backward: the slope at positive logits and at others
+      if (BACKWARD) {
+        const RowRules q = MULTI ? row_rules(r, row) : one;
+        up = q.inv_rep * q.inv_t;
+        down = q.rep * q.inv_t;
+      }
+      constexpr int kTokens = 8;                     // on their way at a time
+      for (int64_t k0 = begin + (int)(MULTI ? tid & (lanes - 1) : tid); k0 < end; k0 += kTokens * lanes) {
+        int64_t tok[kTokens];
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) {
+          const int64_t at = base + min(k0 + j * lanes, (int64_t)end - 1) * r.hist_tok_stride;
+          tok[j] = r.history_bits == 64 ? ((const int64_t *)r.history)[at] : (int64_t)((const int32_t *)r.history)[at];
+        }
+        float l[kTokens];
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) {
+          const bool in_chunk = tok[j] >= c0 && tok[j] < (int64_t)min(a.vocab, c0 + kShapeChunk) && k0 + j * lanes < end;
+          if (!in_chunk) tok[j] = -1;
+          if (BACKWARD) l[j] = in_chunk ? (float)logits[tok[j]] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) {
+          if (tok[j] < 0) continue;
+          unsigned *word = table + table_slot((unsigned)tok[j] - c0 + rl * a.units * 8);
+          if (BACKWARD) *word = __builtin_bit_cast(unsigned, l[j] > 0.f ? up : down);   // the same from every occurrence
+          else if (k0 + j * lanes >= gen) atomicAdd(word, 1u);
+          else atomicOr(word, kPromptOnly);
+        }
       }
     }
     __syncthreads();
-  }
-  const float rep = r.repetition_rows ? r.repetition_rows[row] : r.repetition;
-  const float pres = r.presence_rows ? r.presence_rows[row] : r.presence;
-  const float freq = r.frequency_rows ? r.frequency_rows[row] : r.frequency;
-  const float inv_t = 1.f / (r.temperature_rows ? r.temperature_rows[row] : r.temperature);
-  const float *bias = r.bias ? r.bias + (int64_t)row * r.bias_stride : nullptr;
-  const uint8_t *mask = nullptr;
-  if (r.mask_kind != PPO_XP_MASK_NONE) {
-    const int64_t m = r.mask_row ? r.mask_row[row] : (r.mask_stride == 0 ? 0 : (int64_t)row);
-    if (m >= 0 && m < r.mask_rows) mask = (const uint8_t *)r.mask + m * r.mask_stride * (r.mask_kind == PPO_XP_MASK_BITS ? 4 : 1);
   }
 #pragma unroll
   for (int k = 0; k < kShapeVecs; ++k) {
-    const unsigned e = c0 + (k * 256 + tid) * 8;
-    if (e >= a.vocab) break;
-    const int n = (int)min(8u, a.vocab - e);
-    unsigned allowed = 0xffu;
-    if (mask) {
-      if (r.mask_kind == PPO_XP_MASK_BITS) allowed = mask[e / 8];
-      else {
-        allowed = 0;
-        for (int i = 0; i < n; ++i) allowed |= (mask[e + i] ? 1u : 0u) << i;
+    size_t row; unsigned e;
+    if (!place(k, row, e)) continue;
+    const RowRules q = MULTI ? row_rules(r, row) : one;
+    const unsigned ok = allowed8(q, r.mask_kind, e, a.vocab);
+    u32x4 c[2] = {u32x4(0), u32x4(0)};
+    if (HIST) {
+      c[0] = *(const u32x4 *)(table + (k * 256 + tid) * 4);
+      c[1] = *(const u32x4 *)(table + kShapeChunk / 2 + (k * 256 + tid) * 4);
+    }
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = raw[k].get(i);
+    if (BACKWARD) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= HIST ? __builtin_bit_cast(float, (unsigned)c[i >> 2][i & 3]) : q.inv_t;
+    } else {
+      if (HIST) {
+        const u32x4 some = c[0] | c[1];
+        if (__any((some[0] | some[1] | some[2] | some[3]) != 0)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const unsigned w = c[i >> 2][i & 3];
+            const float n = (float)(w & ~kPromptOnly);
+            x[i] *= w ? (x[i] > 0.f ? q.inv_rep : q.rep) : 1.f;
+            x[i] -= q.freq * n + (n > 0.f ? q.pres : 0.f);
+          }
+        }
       }
+      if (q.bias) {
+        if (e + 8 <= a.vocab) {
+          Raw8<float> b;
+          b.load(q.bias + e);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] += b.get(i);
+        } else {
+          for (int i = 0; i < 8; ++i)
+            if (e + i < a.vocab) x[i] += q.bias[e + i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= q.inv_t;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float x = raw[k].get(i);
-      unsigned c = 0;
-      if (HIST) c = table[e - c0 + i];
-      if (BACKWARD) {
-        x *= inv_t;
-        if (HIST && c && i < n) x = (float)((const T *)a.logits)[(int64_t)row * a.logits_stride + e + i] > 0.f ? x / rep : x * rep;
-        if (!((allowed >> i) & 1)) x = 0.f;
-      } else {
-        if (HIST && c) {
-          x = x > 0.f ? x / rep : x * rep;
-          const unsigned cnt = c & ~kPromptOnly;
-          if (cnt) x -= freq * (float)cnt + pres;
-        }
-        if (bias && i < n) x += bias[e + i];
-        x *= inv_t;
-        if (!((allowed >> i) & 1)) x = -__builtin_inff();
-      }
-      raw[k].set(i, x);
-    }
-    store8(raw[k], out + e, n);
+    for (int i = 0; i < 8; ++i) x[i] = (ok >> i) & 1 ? x[i] : (BACKWARD ? 0.f : -__builtin_inff());
+    raw[k].set8(x);
+    store8(raw[k], (T *)a.out + (int64_t)row * a.out_stride + e, (long)a.vocab - (long)e);
   }
 }
 
@@ -776,28 +889,35 @@ int check_rules(const char *who, const ppo_xp_logit_rules *r, size_t rows, size_
   return 0;
 }
 
+template <typename T, bool HIST, bool BACKWARD>
+void launch_shape(const ShapeArgs &a, dim3 grid, hipStream_t s) {
+  if (a.rows_per > 1) hipLaunchKernelGGL((shape_logits_kernel<T, HIST, BACKWARD, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((shape_logits_kernel<T, HIST, BACKWARD, false>), grid, dim3(256), 0, s, a);
+}
 template <typename T>
 void launch_shape(const ShapeArgs &a, dim3 grid, hipStream_t s, bool hist, bool backward) {
-  if (backward) {
-    if (hist) hipLaunchKernelGGL((shape_logits_kernel<T, true, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((shape_logits_kernel<T, false, true>), grid, dim3(256), 0, s, a);
-  } else {
-    if (hist) hipLaunchKernelGGL((shape_logits_kernel<T, true, false>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((shape_logits_kernel<T, false, false>), grid, dim3(256), 0, s, a);
-  }
+  if (backward) hist ? launch_shape<T, true, true>(a, grid, s) : launch_shape<T, false, true>(a, grid, s);
+  else hist ? launch_shape<T, true, false>(a, grid, s) : launch_shape<T, false, false>(a, grid, s);
 }
 
 int shape(const char *who, int device, void *stream, int dtype, ShapeArgs &a, size_t rows, size_t vocab, const ppo_xp_logit_rules *rules,
           bool backward) {
   if (int rc = check_rules(who, rules, rows, vocab)) return rc;
   if (rows == 0 || vocab == 0) return 0;
+  a.rows = rows;
   a.vocab = (unsigned)vocab;
   a.chunks = (unsigned)((vocab + kShapeChunk - 1) / kShapeChunk);
+  // rows that fill less than half a workgroup's part share one (one workgroup a row: 113 us at 262144 x 32 bf16)
+  a.units = (unsigned)((vocab + 7) / 8);
+  a.rows_per = (unsigned)std::min<size_t>(kShapeChunk / 8 / std::min(a.units, kShapeChunk / 8), rows);
+  a.magic = ((1u << 20) + a.units - 1) / a.units;
+  a.scan_log2 = 8;
+  while (a.scan_log2 && (256u >> a.scan_log2) < a.rows_per) --a.scan_log2;
   a.r = *rules;
   if (rows > kMaxGrid / a.chunks) return ppoxp_fail(PPO_XP_EINVAL, "%s: %zu rows of %zu are too many for one launch", who, rows, vocab);
   DeviceGuard dev(device, who);
   if (dev.rc()) return dev.rc();
-  const dim3 grid((unsigned)(rows * a.chunks));
+  const dim3 grid((unsigned)(a.rows_per > 1 ? (rows + a.rows_per - 1) / a.rows_per : rows * a.chunks));
   const bool hist = rules->history && rules->hist_rows > 0 && rules->hist_len > 0;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == PPO_XP_F32) launch_shape<float>(a, grid, s, hist, backward);
