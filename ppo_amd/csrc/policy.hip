@@ -26,6 +26,7 @@ struct ShapeArgs {
   ppo_xp_logit_rules r;
 };
 
+enum ShapeMode { kForward, kGather, kReadAll };
 constexpr int kShapeVecs = 4;                        // 8-element vectors a thread
 constexpr unsigned kShapeChunk = 256 * 8 * kShapeVecs;
 constexpr unsigned kPromptOnly = 0x80000000u;        // table word: occurrences in the generated part, this bit: in the rest
@@ -74,11 +75,13 @@ __device__ __forceinline__ unsigned allowed8(const RowRules &q, int kind, unsign
 
 // One workgroup shapes one chunk of one row's vocabulary, or several whole rows (MULTI).  With a history it enters the tokens that
 // fall into its part in an LDS table first, while its logits are already on their way into registers: their counts (integer
-// atomics, the order does not matter), or in the backward pass the slope, which every occurrence knows from the token's logit.
+// atomics, the order does not matter), or in the backward pass the slope, which every occurrence knows from the token's logit
+// (kGather), or only that it was seen, where all logits are read (kReadAll).
 // Every workgroup of a row reads the row's whole history; that is cheaper than sorting it while the history is shorter than the
 // vocabulary.  Elements then take their word without a branch: at a seen token in a hundred a wave would enter it anyway.
-template <typename T, bool HIST, bool BACKWARD, bool MULTI>
+template <typename T, bool HIST, int MODE, bool MULTI>
 __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
+  constexpr bool BACKWARD = MODE != kForward;
   __shared__ __attribute__((aligned(16))) unsigned table[HIST ? kShapeChunk : 4];
   const ppo_xp_logit_rules &r = a.r;
   const unsigned tid = threadIdx.x;
@@ -97,29 +100,41 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
     return rl < here;
   };
 
-  Raw8<T> raw[kShapeVecs];
+  auto fetch = [&](Raw8<T> *to, const void *from, int64_t stride) {
 #pragma unroll
-  for (int k = 0; k < kShapeVecs; ++k) {
-    size_t row; unsigned e;
-    const bool live = place(k, row, e);
-    if (live && e + 8 <= a.vocab) {
-      raw[k].load((const T *)a.in + (int64_t)row * a.in_stride + e);
-    } else {                                         // a row's end, or nothing: clamped addresses, no further branch
-      const T *p = (const T *)a.in + (int64_t)(live ? row : row0) * a.in_stride;
-      T q[8];
-      float y[8];
+    for (int k = 0; k < kShapeVecs; ++k) {
+      size_t row; unsigned e;
+      const bool live = place(k, row, e);
+      if (live && e + 8 <= a.vocab) {
+        to[k].load((const T *)from + (int64_t)row * stride + e);
+      } else {                                       // a row's end, or nothing: clamped addresses, no further branch
+        const T *p = (const T *)from + (int64_t)(live ? row : row0) * stride;
+        T q[8];
+        float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = p[min(e + i, a.vocab - 1)];
+        for (int i = 0; i < 8; ++i) q[i] = p[min(e + i, a.vocab - 1)];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = (float)q[i];
-      raw[k].set8(y);
+        for (int i = 0; i < 8; ++i) y[i] = (float)q[i];
+        to[k].set8(y);
+      }
+    }
+  };
+  Raw8<T> raw[kShapeVecs], own[MODE == kReadAll ? kShapeVecs : 1];
+  fetch(raw, a.in, a.in_stride);
+  if (MODE == kReadAll) fetch(own, a.logits, a.logits_stride);
+  unsigned ok[kShapeVecs];                           // with one row a workgroup the mask's bits are on their way as well
+  if (!MULTI) {
+#pragma unroll
+    for (int k = 0; k < kShapeVecs; ++k) {
+      const unsigned e = c0 + (k * 256 + tid) * 8;
+      ok[k] = one.mask && r.mask_kind == PPO_XP_MASK_BITS ? one.mask[min(e, a.vocab - 1) / 8] : 0xffu;
     }
   }
   if (HIST) {
 #pragma unroll
     for (int k = 0; k < kShapeVecs; ++k) {
       unsigned word = 0;
-      if (BACKWARD) {
+      if (MODE == kGather) {
         float inv_t = one.inv_t;
         if (MULTI) {
           size_t row; unsigned e;
@@ -141,9 +156,9 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
       const int begin = r.hist_begin ? max(r.hist_begin[row], 0) : 0;
       const int gen = r.gen_begin ? r.gen_begin[row] : begin;
       const int64_t base = h * r.hist_row_stride;
-      const T *logits = BACKWARD ? (const T *)a.logits + (int64_t)row * a.logits_stride : nullptr;
+      const T *logits = MODE == kGather ? (const T *)a.logits + (int64_t)row * a.logits_stride : nullptr;
       float up = 0.f, down = 0.f;                    // backward: the slope at positive logits and at others
-      if (BACKWARD) {
+      if (MODE == kGather) {
         const RowRules q = MULTI ? row_rules(r, row) : one;
         up = q.inv_rep * q.inv_t;
         down = q.rep * q.inv_t;
@@ -161,13 +176,14 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
         for (int j = 0; j < kTokens; ++j) {
           const bool in_chunk = tok[j] >= c0 && tok[j] < (int64_t)min(a.vocab, c0 + kShapeChunk) && k0 + j * lanes < end;
           if (!in_chunk) tok[j] = -1;
-          if (BACKWARD) l[j] = in_chunk ? (float)logits[tok[j]] : 0.f;
+          if (MODE == kGather) l[j] = in_chunk ? (float)logits[tok[j]] : 0.f;
         }
 #pragma unroll
         for (int j = 0; j < kTokens; ++j) {
           if (tok[j] < 0) continue;
           unsigned *word = table + table_slot((unsigned)tok[j] - c0 + rl * a.units * 8);
-          if (BACKWARD) *word = __builtin_bit_cast(unsigned, l[j] > 0.f ? up : down);   // the same from every occurrence
+          if (MODE == kGather) *word = __builtin_bit_cast(unsigned, l[j] > 0.f ? up : down);   // the same from every occurrence
+          else if (MODE == kReadAll) *word = 1;
           else if (k0 + j * lanes >= gen) atomicAdd(word, 1u);
           else atomicOr(word, kPromptOnly);
         }
@@ -180,7 +196,7 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
     size_t row; unsigned e;
     if (!place(k, row, e)) continue;
     const RowRules q = MULTI ? row_rules(r, row) : one;
-    const unsigned ok = allowed8(q, r.mask_kind, e, a.vocab);
+    const unsigned allowed = !MULTI && r.mask_kind != PPO_XP_MASK_BYTES ? ok[k] : allowed8(q, r.mask_kind, e, a.vocab);
     u32x4 c[2] = {u32x4(0), u32x4(0)};
     if (HIST) {
       c[0] = *(const u32x4 *)(table + (k * 256 + tid) * 4);
@@ -191,7 +207,11 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
     for (int i = 0; i < 8; ++i) x[i] = raw[k].get(i);
     if (BACKWARD) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= HIST ? __builtin_bit_cast(float, (unsigned)c[i >> 2][i & 3]) : q.inv_t;
+      for (int i = 0; i < 8; ++i) {
+        const unsigned w = c[i >> 2][i & 3];
+        if (MODE == kReadAll) x[i] *= q.inv_t * (w ? (own[k].get(i) > 0.f ? q.inv_rep : q.rep) : 1.f);
+        else x[i] *= HIST ? __builtin_bit_cast(float, w) : q.inv_t;
+      }
     } else {
       if (HIST) {
         const u32x4 some = c[0] | c[1];
@@ -220,7 +240,7 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
       for (int i = 0; i < 8; ++i) x[i] *= q.inv_t;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (ok >> i) & 1 ? x[i] : (BACKWARD ? 0.f : -__builtin_inff());
+    for (int i = 0; i < 8; ++i) x[i] = (allowed >> i) & 1 ? x[i] : (BACKWARD ? 0.f : -__builtin_inff());
     raw[k].set8(x);
     store8(raw[k], (T *)a.out + (int64_t)row * a.out_stride + e, (long)a.vocab - (long)e);
   }
@@ -889,15 +909,19 @@ int check_rules(const char *who, const ppo_xp_logit_rules *r, size_t rows, size_
   return 0;
 }
 
-template <typename T, bool HIST, bool BACKWARD>
+template <typename T, bool HIST, int MODE>
 void launch_shape(const ShapeArgs &a, dim3 grid, hipStream_t s) {
-  if (a.rows_per > 1) hipLaunchKernelGGL((shape_logits_kernel<T, HIST, BACKWARD, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((shape_logits_kernel<T, HIST, BACKWARD, false>), grid, dim3(256), 0, s, a);
+  if (a.rows_per > 1) hipLaunchKernelGGL((shape_logits_kernel<T, HIST, MODE, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((shape_logits_kernel<T, HIST, MODE, false>), grid, dim3(256), 0, s, a);
 }
 template <typename T>
 void launch_shape(const ShapeArgs &a, dim3 grid, hipStream_t s, bool hist, bool backward) {
-  if (backward) hist ? launch_shape<T, true, true>(a, grid, s) : launch_shape<T, false, true>(a, grid, s);
-  else hist ? launch_shape<T, true, false>(a, grid, s) : launch_shape<T, false, false>(a, grid, s);
+  if (!backward) hist ? launch_shape<T, true, kForward>(a, grid, s) : launch_shape<T, false, kForward>(a, grid, s);
+  else if (!hist) launch_shape<T, false, kGather>(a, grid, s);
+  // Fetching the logits of seen tokens one by one costs more than reading them all from about a token in 30 on (2048 x 50001 bf16:
+  // 22, 48 and 87 us beside 43 at 1024, 2048 and 4096 tokens a row); histories are taken to be half full.
+  else if ((uint64_t)a.r.hist_len * 16 < a.vocab) launch_shape<T, true, kGather>(a, grid, s);
+  else launch_shape<T, true, kReadAll>(a, grid, s);
 }
 
 int shape(const char *who, int device, void *stream, int dtype, ShapeArgs &a, size_t rows, size_t vocab, const ppo_xp_logit_rules *rules,
