@@ -918,9 +918,9 @@ template <typename T>
 void launch_shape(const ShapeArgs &a, dim3 grid, hipStream_t s, bool hist, bool backward) {
   if (!backward) hist ? launch_shape<T, true, kForward>(a, grid, s) : launch_shape<T, false, kForward>(a, grid, s);
   else if (!hist) launch_shape<T, false, kGather>(a, grid, s);
-  // Fetching the logits of seen tokens one by one costs more than reading them all from about a token in 30 on (2048 x 50001 bf16:
-  // 22, 48 and 87 us beside 43 at 1024, 2048 and 4096 tokens a row); histories are taken to be half full.
-  else if ((uint64_t)a.r.hist_len * 16 < a.vocab) launch_shape<T, true, kGather>(a, grid, s);
+  // Fetching the logits of seen tokens one by one costs as much as reading them all at about a token in 50 (2048 x 50001 bf16, us one
+  // by one against all: 133 and 132 at 1024 tokens a row, 164 and 134 at 2048, 232 and 157 at 4096); histories may be partly filled.
+  else if ((uint64_t)a.r.hist_len * 32 < a.vocab) launch_shape<T, true, kGather>(a, grid, s);
   else launch_shape<T, true, kReadAll>(a, grid, s);
 }
 
