@@ -143,6 +143,11 @@ __device__ __forceinline__ float group_max_nan(float x, unsigned lanes) {
 __device__ __forceinline__ float group_sum(float x, unsigned lanes) {
   return group_reduce(x, lanes, [](float a, float b) { return a + b; });
 }
+__device__ __forceinline__ unsigned group_max_bits(unsigned x, unsigned lanes) {   // of bit patterns, as integers
+  return __builtin_bit_cast(unsigned, group_reduce(__builtin_bit_cast(float, x), lanes, [](float a, float b) {
+    return __builtin_bit_cast(float, max(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)));
+  }));
+}
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);

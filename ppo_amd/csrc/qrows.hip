@@ -14,6 +14,29 @@ typedef u32x2 u32x2_a1 __attribute__((aligned(1)));
 typedef unsigned u32_a1 __attribute__((aligned(1)));
 typedef unsigned short u16_a1 __attribute__((aligned(1)));
 
+// Units of a launch (16 bytes of output or 8 elements) lie row after row, `slots` to a row; a workgroup takes 256 * U of them.
+struct Units {
+  size_t total, row0;
+  unsigned slots, off;       // the workgroup's first unit is unit `off` of row0
+  float inv;
+  __device__ __forceinline__ Units(size_t total_, unsigned slots_, unsigned per_block) : total(total_), slots(slots_) {
+    const size_t first = (size_t)blockIdx.x * per_block;
+    row0 = total >> 32 ? first / slots : (unsigned)first / slots;
+    off = (unsigned)(first - row0 * slots);
+    inv = 1.f / (float)slots;
+  }
+  // Unit k * 256 + thread: its row and its place there; false beyond the last one.  (Exact: off + k * 256 + thread < 2^24.)
+  __device__ __forceinline__ bool at(int k, size_t &row, unsigned &slot) const {
+    const unsigned t = off + k * 256 + threadIdx.x;
+    unsigned q = (unsigned)((float)t * inv), r = t - q * slots;
+    if ((int)r < 0) { --q; r += slots; }
+    if (r >= slots) { ++q; r -= slots; }
+    row = row0 + q;
+    slot = r;
+    return (row0 * slots + t) < total;
+  }
+};
+
 struct QuantArgs {
   const void *rows;
   uint8_t *codes;
@@ -38,71 +61,88 @@ __device__ __forceinline__ int round_quotient(float x, float s, float inv, float
 
 // One lane holds 8 elements, group / 8 neighbouring lanes one group: the group's largest magnitude is found with lane
 // shuffles and the row is read once.  Magnitudes are compared as integers, which puts NaN and inf above every number.
-template <typename T, int FORMAT>
+template <typename T, int FORMAT, int U>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
-  const size_t first = (size_t)blockIdx.x * 256;
-  const size_t row0 = first / a.slots;
-  const unsigned t = (unsigned)(first - row0 * a.slots) + threadIdx.x;
-  const bool live = first + threadIdx.x < a.total;
-  const size_t row = row0 + t / a.slots;
-  const unsigned e = (t % a.slots) * 8;
-  const long left = live ? (long)a.width - (long)e : 0;
-  Raw8<T> raw;
-  load8(raw, (const T *)a.rows + (int64_t)row * a.rows_stride + e, left, 0.f);
-  float x[8];
-  unsigned top = 0;
+  const Units units(a.total, a.slots, 256 * U);
+  Raw8<T> raw[U];
+  size_t row[U];
+  unsigned e[U], top[U];
+  long left[U];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = raw.get(i);
-    top = max(top, __builtin_bit_cast(unsigned, x[i]) & 0x7fffffffu);
-  }
-  for (unsigned off = 1; off < (1u << a.lanes_log2); off <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, (int)off, 64));
-
-  const bool empty = top < (17u << 23), bad = top >= 0x7f800000u;   // below 2^-110 | NaN or inf
-  float s, inv;
-  if (FORMAT == PPO_XP_Q_E4M3) {
-    // top = 1.m 2^E <= 448 2^k = 1.75 2^(8+k)
-    const unsigned k127 = (top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-    s = __builtin_bit_cast(float, k127 << 23);
-    inv = __builtin_bit_cast(float, (254 - k127) << 23);
-  } else {
-    s = __builtin_bit_cast(float, top) / (FORMAT == PPO_XP_Q_INT8 ? 127.f : 7.f);
-    inv = 1.f / s;
-  }
-  if (empty || bad) { s = bad ? __builtin_nanf("") : 0.f; inv = 0.f; }
-  if (left > 0 && ((t % a.slots) & ((1u << a.lanes_log2) - 1)) == 0)
-    a.scales[(int64_t)(a.at + row) * a.scales_stride + (e >> (a.lanes_log2 + 3))] = s;
-
-  if (left <= 0) return;
-  uint8_t *dst = a.codes + (int64_t)(a.at + row) * a.codes_stride;
-  if (FORMAT == PPO_XP_Q_INT4) {
-    unsigned w = 0;
-    if (inv != 0.f) {
+  for (int k = 0; k < U; ++k) {
+    const bool live = units.at(k, row[k], e[k]);
+    e[k] *= 8;
+    left[k] = live ? (long)a.width - (long)e[k] : 0;
+    const T *p = (const T *)a.rows + (int64_t)row[k] * a.rows_stride;
+    if (left[k] >= 8) {
+      raw[k].load(p + e[k]);
+    } else {                                           // a row's end, or beyond it: clamped addresses, no further branch
+      p = (const T *)a.rows + (int64_t)(live ? row[k] : 0) * a.rows_stride;
+      T q[8];
+      float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w |= ((unsigned)round_quotient(x[i], s, inv, 0.5f * s) & 15u) << (4 * i);
+      for (int i = 0; i < 8; ++i) q[i] = p[min(e[k] + i, a.width - 1)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = i < left[k] ? (float)q[i] : 0.f;
+      raw[k].set8(y);
     }
-    dst += e / 2;
-    if (left >= 8) *(u32_a1 *)dst = w;
-    else for (int i = 0; i < (int)(left + 1) / 2; ++i) dst[i] = (uint8_t)(w >> (8 * i));
-    return;
   }
-  u32x2 w = {0, 0};
-  if (inv != 0.f) {
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    top[k] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top[k] = max(top[k], __builtin_bit_cast(unsigned, raw[k].get(i)) & 0x7fffffffu);
+    top[k] = group_max_bits(top[k], 1u << a.lanes_log2);
+  }
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const bool empty = top[k] < (17u << 23), bad = top[k] >= 0x7f800000u;   // below 2^-110 | NaN or inf
+    float s, inv;
     if (FORMAT == PPO_XP_Q_E4M3) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        int p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * h] * inv, x[4 * h + 1] * inv, 0, false);
-        p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * h + 2] * inv, x[4 * h + 3] * inv, p, true);
-        w[h] = (unsigned)p;
-      }
+      // top = 1.m 2^E <= 448 2^k = 1.75 2^(8+k)
+      const unsigned k127 = (top[k] >> 23) - 8 + ((top[k] & 0x7fffffu) > 0x600000u ? 1 : 0);
+      s = __builtin_bit_cast(float, k127 << 23);
+      inv = __builtin_bit_cast(float, (254 - k127) << 23);
     } else {
+      s = __builtin_bit_cast(float, top[k]) / (FORMAT == PPO_XP_Q_INT8 ? 127.f : 7.f);
+      inv = 1.f / s;
+    }
+    if (empty || bad) { s = bad ? __builtin_nanf("") : 0.f; inv = 0.f; }
+    if (left[k] <= 0) continue;
+    if (((e[k] >> 3) & ((1u << a.lanes_log2) - 1)) == 0)
+      a.scales[(int64_t)(a.at + row[k]) * a.scales_stride + (e[k] >> (a.lanes_log2 + 3))] = s;
+    uint8_t *dst = a.codes + (int64_t)(a.at + row[k]) * a.codes_stride;
+    u32x2 w = {0, 0};
+    if (inv != 0.f) {
+      if (FORMAT == PPO_XP_Q_E4M3) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i >> 2] |= ((unsigned)round_quotient(x[i], s, inv, 0.5f * s) & 255u) << (8 * (i & 3));
+        for (int h = 0; h < 2; ++h) {
+          int p = __builtin_amdgcn_cvt_pk_fp8_f32(raw[k].get(4 * h) * inv, raw[k].get(4 * h + 1) * inv, 0, false);
+          p = __builtin_amdgcn_cvt_pk_fp8_f32(raw[k].get(4 * h + 2) * inv, raw[k].get(4 * h + 3) * inv, p, true);
+          w[h] = (unsigned)p;
+        }
+      } else {
+        const float half = 0.5f * s;
+        int q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = round_quotient(raw[k].get(i), s, inv, half);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (FORMAT == PPO_XP_Q_INT4) w[0] |= ((unsigned)q[i] & 15u) << (4 * i);
+          else w[i >> 2] |= ((unsigned)q[i] & 255u) << (8 * (i & 3));
+        }
+      }
+    }
+    if (FORMAT == PPO_XP_Q_INT4) {
+      dst += e[k] / 2;
+      if (left[k] >= 8) *(u32_a1 *)dst = w[0];
+      else for (int i = 0; i < (int)(left[k] + 1) / 2; ++i) dst[i] = (uint8_t)(w[0] >> (8 * i));
+    } else {
+      dst += e[k];
+      if (left[k] >= 8) *(u32x2_a1 *)dst = w;
+      else for (int i = 0; i < (int)left[k]; ++i) dst[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
     }
   }
-  dst += e;
-  if (left >= 8) *(u32x2_a1 *)dst = w;
-  else for (int i = 0; i < (int)left; ++i) dst[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
 }
 
 struct DequantArgs {
@@ -115,58 +155,86 @@ struct DequantArgs {
   unsigned width, slots, group_log2, index_bits;      // slots of 16 / sizeof(T) elements per row
 };
 
-template <int FORMAT>
-__device__ __forceinline__ void decode4(const uint8_t *p, int left, float v[4]) {   // 4 codes from element 0 of p on
-  unsigned w = 0;
-  if (FORMAT == PPO_XP_Q_INT4) {
-    if (left >= 4) w = *(const u16_a1 *)p;
-    else for (int i = 0; i < (left + 1) / 2; ++i) w |= (unsigned)p[i] << (8 * i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)((int)(w << (28 - 4 * i)) >> 28);
-    return;
+// N codes from element 0 of p on (N 4 or 8, p at an even element), as they lie: 4 bits or 8 each.
+template <int FORMAT, int N>
+struct Codes {
+  static constexpr int kBits = FORMAT == PPO_XP_Q_INT4 ? 4 : 8, kBytes = N * kBits / 8;
+  unsigned w[kBytes > 4 ? 2 : 1];
+  __device__ __forceinline__ void load(const uint8_t *p) {
+    if constexpr (kBytes == 8) { const u32x2 v = *(const u32x2_a1 *)p; w[0] = v.x; w[1] = v.y; }
+    else if constexpr (kBytes == 4) w[0] = *(const u32_a1 *)p;
+    else w[0] = *(const u16_a1 *)p;
   }
-  if (left >= 4) w = *(const u32_a1 *)p;
-  else for (int i = 0; i < left; ++i) w |= (unsigned)p[i] << (8 * i);
-  if (FORMAT == PPO_XP_Q_INT8) {
+  __device__ __forceinline__ void load(const uint8_t *p, int left) {   // `left` elements, at least one; what is beyond is not read
+    const int last = (left * kBits + 7) / 8 - 1;
+    unsigned b[kBytes];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)((int)(w << (24 - 8 * i)) >> 24);
-  } else {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-    v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
+    for (int i = 0; i < kBytes; ++i) b[i] = p[min(i, last)];
+#pragma unroll
+    for (unsigned &x : w) x = 0;
+#pragma unroll
+    for (int i = 0; i < kBytes; ++i) w[i / 4] |= b[i] << (8 * (i % 4));
   }
-}
+  __device__ __forceinline__ void values(float v[N]) const {
+    if constexpr (FORMAT == PPO_XP_Q_E4M3) {
+      typedef float f2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int h = 0; h < N / 4; ++h) {
+        const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], true);
+        v[4 * h] = lo.x; v[4 * h + 1] = lo.y; v[4 * h + 2] = hi.x; v[4 * h + 3] = hi.y;
+      }
+    } else {
+      constexpr int kPer = 32 / kBits;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = (float)((int)(w[i / kPer] << (32 - kBits - kBits * (i % kPer))) >> (32 - kBits));
+    }
+  }
+};
 
-// One lane writes 16 bytes of output.  An index beyond the store reads its last row, as the gathers of a pass do.
-template <typename T, int FORMAT>
+// One lane writes U times 16 bytes of output, its index entries, codes and scales on their way together.  An index beyond the store
+// reads its last row, as the gathers of a pass do.
+template <typename T, int FORMAT, int U>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(DequantArgs a) {
   constexpr int E = 16 / sizeof(T);
-  const size_t first = (size_t)blockIdx.x * 256;
-  if (first + threadIdx.x >= a.total) return;
-  const size_t row0 = first / a.slots;
-  const unsigned t = (unsigned)(first - row0 * a.slots) + threadIdx.x;
-  const size_t row = row0 + t / a.slots;
-  const unsigned e = (t % a.slots) * E;
-  size_t src = a.at + row;
-  if (a.index) src = a.index_bits == 32 ? (size_t)((const uint32_t *)a.index)[row] : (size_t)((const uint64_t *)a.index)[row];
-  src = min(src, a.store_rows - 1);
-  const int left = (int)(a.width - e);
-  const float s = a.scales[(int64_t)src * a.scales_stride + (e >> a.group_log2)];
-  const uint8_t *p = a.codes + (int64_t)src * a.codes_stride + (FORMAT == PPO_XP_Q_INT4 ? e / 2 : e);
-  T *dst = (T *)a.out + (int64_t)row * a.out_stride + e;
-  float v[E];
+  const Units units(a.total, a.slots, 256 * U);
+  size_t row[U], src[U];
+  unsigned e[U];
+  bool live[U];
 #pragma unroll
-  for (int h = 0; h < E / 4; ++h) decode4<FORMAT>(p + h * (FORMAT == PPO_XP_Q_INT4 ? 2 : 4), left - 4 * h, v + 4 * h);
-  if (left >= E) {
-    typedef T vec __attribute__((ext_vector_type(E)));
-    typedef vec vec_u __attribute__((aligned(sizeof(T))));
-    vec o;
+  for (int k = 0; k < U; ++k) {
+    live[k] = units.at(k, row[k], e[k]);
+    e[k] *= E;
+    if (!live[k]) { row[k] = 0; e[k] = 0; }
+    src[k] = a.at + row[k];
+    if (a.index) src[k] = a.index_bits == 32 ? (size_t)((const uint32_t *)a.index)[row[k]] : (size_t)((const uint64_t *)a.index)[row[k]];
+  }
+  Codes<FORMAT, E> codes[U];
+  float s[U];
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = (T)(v[i] * s);
-    *(vec_u *)dst = o;
-  } else {
-    for (int i = 0; i < E; ++i)
-      if (i < left) dst[i] = (T)(v[i] * s);
+  for (int k = 0; k < U; ++k) {
+    src[k] = min(src[k], a.store_rows - 1);
+    const uint8_t *p = a.codes + (int64_t)src[k] * a.codes_stride + (FORMAT == PPO_XP_Q_INT4 ? e[k] / 2 : e[k]);
+    s[k] = a.scales[(int64_t)src[k] * a.scales_stride + (e[k] >> a.group_log2)];
+    if (e[k] + E <= a.width) codes[k].load(p);
+    else codes[k].load(p, (int)(a.width - e[k]));
+  }
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    if (!live[k]) continue;
+    T *dst = (T *)a.out + (int64_t)row[k] * a.out_stride + e[k];
+    float v[E];
+    codes[k].values(v);
+    if (e[k] + E <= a.width) {
+      typedef T vec __attribute__((ext_vector_type(E)));
+      typedef vec vec_u __attribute__((aligned(sizeof(T))));
+      vec o;
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] = (T)(v[i] * s[k]);
+      *(vec_u *)dst = o;
+    } else {
+      for (int i = 0; i < E; ++i)
+        if (e[k] + i < a.width) dst[i] = (T)(v[i] * s[k]);
+    }
   }
 }
 
@@ -191,17 +259,32 @@ int check_store(const char *who, int dtype, size_t width, int format, size_t gro
   return 0;
 }
 
-template <typename T>
-void launch_quant(int format, dim3 grid, hipStream_t s, const QuantArgs &a) {
-  if (format == PPO_XP_Q_INT8) hipLaunchKernelGGL((quantize_rows_kernel<T, PPO_XP_Q_INT8>), grid, dim3(256), 0, s, a);
-  else if (format == PPO_XP_Q_E4M3) hipLaunchKernelGGL((quantize_rows_kernel<T, PPO_XP_Q_E4M3>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((quantize_rows_kernel<T, PPO_XP_Q_INT4>), grid, dim3(256), 0, s, a);
+// Four units a lane hide the latency of large calls (a small one would not reach every CU).
+constexpr size_t kManyUnits = size_t(256) * 256 * 4;
+
+template <typename T, int U>
+void launch_quant(int format, hipStream_t s, const QuantArgs &a) {
+  const dim3 grid((unsigned)((a.total + 256 * U - 1) / (256 * U)));
+  if (format == PPO_XP_Q_INT8) hipLaunchKernelGGL((quantize_rows_kernel<T, PPO_XP_Q_INT8, U>), grid, dim3(256), 0, s, a);
+  else if (format == PPO_XP_Q_E4M3) hipLaunchKernelGGL((quantize_rows_kernel<T, PPO_XP_Q_E4M3, U>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((quantize_rows_kernel<T, PPO_XP_Q_INT4, U>), grid, dim3(256), 0, s, a);
 }
 template <typename T>
-void launch_dequant(int format, dim3 grid, hipStream_t s, const DequantArgs &a) {
-  if (format == PPO_XP_Q_INT8) hipLaunchKernelGGL((dequantize_rows_kernel<T, PPO_XP_Q_INT8>), grid, dim3(256), 0, s, a);
-  else if (format == PPO_XP_Q_E4M3) hipLaunchKernelGGL((dequantize_rows_kernel<T, PPO_XP_Q_E4M3>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((dequantize_rows_kernel<T, PPO_XP_Q_INT4>), grid, dim3(256), 0, s, a);
+void launch_quant(int format, hipStream_t s, const QuantArgs &a) {
+  if (a.total >= kManyUnits) launch_quant<T, 4>(format, s, a);
+  else launch_quant<T, 1>(format, s, a);
+}
+template <typename T, int U>
+void launch_dequant(int format, hipStream_t s, const DequantArgs &a) {
+  const dim3 grid((unsigned)((a.total + 256 * U - 1) / (256 * U)));
+  if (format == PPO_XP_Q_INT8) hipLaunchKernelGGL((dequantize_rows_kernel<T, PPO_XP_Q_INT8, U>), grid, dim3(256), 0, s, a);
+  else if (format == PPO_XP_Q_E4M3) hipLaunchKernelGGL((dequantize_rows_kernel<T, PPO_XP_Q_E4M3, U>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((dequantize_rows_kernel<T, PPO_XP_Q_INT4, U>), grid, dim3(256), 0, s, a);
+}
+template <typename T>
+void launch_dequant(int format, hipStream_t s, const DequantArgs &a) {
+  if (a.total >= kManyUnits) launch_dequant<T, 4>(format, s, a);
+  else launch_dequant<T, 1>(format, s, a);
 }
 
 }  // namespace
@@ -227,11 +310,10 @@ int ppo_xp_quantize_rows(int device, void *stream, int dtype, const void *rows, 
   a.total = n * a.slots;
   DeviceGuard dev(device, "quantize_rows");
   if (dev.rc()) return dev.rc();
-  const dim3 grid((unsigned)((a.total + 255) / 256));
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == PPO_XP_F32) launch_quant<float>(format, grid, s, a);
-  else if (dtype == PPO_XP_BF16) launch_quant<__bf16>(format, grid, s, a);
-  else launch_quant<_Float16>(format, grid, s, a);
+  if (dtype == PPO_XP_F32) launch_quant<float>(format, s, a);
+  else if (dtype == PPO_XP_BF16) launch_quant<__bf16>(format, s, a);
+  else launch_quant<_Float16>(format, s, a);
   return launched("quantize_rows");
 }
 
@@ -258,11 +340,10 @@ int ppo_xp_dequantize_rows(int device, void *stream, int dtype, const void *code
   a.total = n * a.slots;
   DeviceGuard dev(device, "dequantize_rows");
   if (dev.rc()) return dev.rc();
-  const dim3 grid((unsigned)((a.total + 255) / 256));
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == PPO_XP_F32) launch_dequant<float>(format, grid, s, a);
-  else if (dtype == PPO_XP_BF16) launch_dequant<__bf16>(format, grid, s, a);
-  else launch_dequant<_Float16>(format, grid, s, a);
+  if (dtype == PPO_XP_F32) launch_dequant<float>(format, s, a);
+  else if (dtype == PPO_XP_BF16) launch_dequant<__bf16>(format, s, a);
+  else launch_dequant<_Float16>(format, s, a);
   return launched("dequantize_rows");
 }
 
