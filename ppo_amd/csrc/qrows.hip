@@ -192,7 +192,8 @@ struct Codes {
 };
 
 // One lane writes U times 16 bytes of output, its index entries, codes and scales on their way together.  An index beyond the store
-// reads its last row, as the gathers of a pass do.
+// reads its last row, as the gathers of a pass do.  The output goes past the caches, which keep the store (16384 x 4100 int4 to bf16:
+// 35 us, through them 46).
 template <typename T, int FORMAT, int U>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(DequantArgs a) {
   constexpr int E = 16 / sizeof(T);
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(DequantArgs a) {
       vec o;
 #pragma unroll
       for (int i = 0; i < E; ++i) o[i] = (T)(v[i] * s[k]);
-      *(vec_u *)dst = o;
+      __builtin_nontemporal_store(o, (vec_u *)dst);
     } else {
       for (int i = 0; i < E; ++i)
         if (e[k] + i < a.width) dst[i] = (T)(v[i] * s[k]);
@@ -259,7 +260,8 @@ int check_store(const char *who, int dtype, size_t width, int format, size_t gro
   return 0;
 }
 
-// Four units a lane hide the latency of large calls (a small one would not reach every CU).
+// Several units a lane hide the latency of large calls (a small one would not reach every CU): two where rows are read whole (32768 x
+// 4096 bf16: 70 us, with four 88, with one 83), four where they are gathered.
 constexpr size_t kManyUnits = size_t(256) * 256 * 4;
 
 template <typename T, int U>
@@ -271,7 +273,7 @@ void launch_quant(int format, hipStream_t s, const QuantArgs &a) {
 }
 template <typename T>
 void launch_quant(int format, hipStream_t s, const QuantArgs &a) {
-  if (a.total >= kManyUnits) launch_quant<T, 4>(format, s, a);
+  if (a.total >= kManyUnits) launch_quant<T, 2>(format, s, a);
   else launch_quant<T, 1>(format, s, a);
 }
 template <typename T, int U>
