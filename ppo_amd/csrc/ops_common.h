@@ -50,7 +50,9 @@ struct Raw8 {
     const unsigned h = __builtin_bit_cast(unsigned short, (T)x);
     v[i >> 1] = (i & 1) ? ((v[i >> 1] & 0xffffu) | (h << 16)) : ((v[i >> 1] & 0xffff0000u) | h);
   }
-  __device__ __forceinline__ void store(T *p) const { *(u32x4_a2 *)p = v; }
+  // Past the caches: whole lines from a wave, which nothing here reads again (5 % at 4096 x 65536).  The halves of eight floats fill
+  // lines in two instructions and lose a third that way.
+  __device__ __forceinline__ void store(T *p) const { __builtin_nontemporal_store(v, (u32x4_a2 *)p); }
   __device__ __forceinline__ void set8(const float y[8]) {
     typedef T pair __attribute__((ext_vector_type(2)));
 #pragma unroll
