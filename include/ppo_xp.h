@@ -385,7 +385,7 @@ int ppo_xp_action_stats(int device, void *stream, int dtype, const void *logits,
                         const int64_t *actions, float *neglogps, float *entropies, size_t rows, size_t vocab,
                         void *workspace, size_t workspace_bytes);
 /* Bytes of workspace that ppo_xp_action_stats (loss = 0) or ppo_xp_policy_loss (loss = 1) needs for these sizes; 0: none. */
-size_t ppo_xp_policy_workspace(int dtype, size_t rows, size_t vocab, int loss);
+size_t ppo_xp_policy_workspace(size_t rows, size_t vocab, int loss);
 
 /* The streams of a gathered minibatch (ppo_batch_view) and the critic's new values, [rows] each. */
 typedef struct ppo_xp_policy_batch {

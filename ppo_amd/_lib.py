@@ -110,7 +110,7 @@ SYMBOLS = {
     "ppo_xp_shape_logits": (_i, [_i, _vp, _i, _vp, _i64, _vp, _i64, _sz, _sz, _vp]),
     "ppo_xp_shape_logits_backward": (_i, [_i, _vp, _i, _vp, _i64, _vp, _i64, _vp, _i64, _sz, _sz, _vp]),
     "ppo_xp_action_stats": (_i, [_i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _sz, _sz, _vp, _sz]),
-    "ppo_xp_policy_workspace": (_sz, [_i, _sz, _sz, _i]),
+    "ppo_xp_policy_workspace": (_sz, [_sz, _sz, _i]),
     "ppo_xp_policy_loss": (_i, [_i, _vp, _i, _vp, _i64, _vp, _f, _f, _f, _d, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz]),
     "ppo_xp_quantize_rows": (_i, [_i, _vp, _i, _vp, _i64, _sz, _sz, _i, _sz, _vp, _i64, _vp, _i64, _sz, _sz]),
     "ppo_xp_dequantize_rows": (_i, [_i, _vp, _i, _vp, _i64, _vp, _i64, _sz, _sz, _i, _sz, _vp, _i, _sz, _sz, _vp, _i64]),

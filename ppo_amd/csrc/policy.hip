@@ -678,8 +678,8 @@ __global__ __launch_bounds__(256, 4) void policy_group_kernel(PolicyArgs a, unsi
 }
 
 // One workgroup per row, statistics only: the row streams through registers once, a few vectors a thread at a time.
-template <typename T, int kStatsVecs>
-__global__ __launch_bounds__(256) void policy_stats_row_kernel(PolicyArgs a) {
+template <typename T, int THREADS, int kStatsVecs>
+__global__ __launch_bounds__(THREADS) void policy_stats_row_kernel(PolicyArgs a) {
   __shared__ Softmax red[16];
   const size_t row = blockIdx.x;
   const T *in = (const T *)a.logits + (int64_t)row * a.stride;
@@ -688,12 +688,12 @@ __global__ __launch_bounds__(256) void policy_stats_row_kernel(PolicyArgs a) {
   const Span at = span_of(in, a.vocab);
   Softmax w{-__builtin_inff(), 0.f, 0.f};
   if (action != -1)
-    for (unsigned e0 = 0; e0 < at.end; e0 += kStatsVecs * 2048) {
+    for (unsigned e0 = 0; e0 < at.end; e0 += kStatsVecs * THREADS * 8) {
       Raw8<T> r[kStatsVecs];
-      const Span part{e0 ? 0u : at.first, min(at.end - e0, kStatsVecs * 2048u)};
-      load_row<kStatsVecs>(r, in + e0, threadIdx.x, 256, part);
+      const Span part{e0 ? 0u : at.first, min(at.end - e0, kStatsVecs * THREADS * 8u)};
+      load_row<kStatsVecs>(r, in + e0, threadIdx.x, THREADS, part);
       Softmax q{-__builtin_inff(), 0.f, 0.f};
-      row_softmax<kStatsVecs>(q, r, in + e0, threadIdx.x * 8, 2048, part);
+      row_softmax<kStatsVecs>(q, r, in + e0, threadIdx.x * 8, THREADS * 8, part);
       const float m = __builtin_elementwise_maximum(w.m, q.m);
       rebase(w.m, m, w.s, w.t);
       rebase(q.m, m, q.s, q.t);
@@ -961,17 +961,20 @@ struct Plan {
   size_t o_slices = 0, o_ticket = 0, o_parts = 0, o_picked = 0, bytes = 0;
 };
 
-// Few rows leave most of the 256 CUs idle with one workgroup each; the split costs a launch and a second read out of the caches.
-constexpr size_t kSplitRows = 256, kSplitVocab = 2 * kSplitChunk;
+// Few long rows leave most of the 256 CUs idle with a workgroup each; the split costs a launch more (4 us of the host's time) and a
+// second read out of the caches.  Measured in us a call, one workgroup a row | split: statistics of 8 x 131072 f32 9.0 | 12.5,
+// 8 x 262144 f32 16.4 | 12.5, 200 x 262144 f32 32.4 | 33.7; objective of 8 x 65536 bf16 17.5 | 20.3, 8 x 131072 f32 27.4 | 20.2,
+// 200 x 131072 bf16 26.0 | 33.5.
+constexpr size_t kSplitRows = 128, kSplitLoss = 65536, kSplitStats = 131072;   // rows, tokens
 
-Plan plan_of(int dtype, size_t rows, size_t vocab, bool loss) {
+Plan plan_of(size_t rows, size_t vocab, bool loss) {
   Plan p;
   if (vocab <= kGroupVocab) {
     p.route = vocab <= kSmallVocab ? kSmall : kGroup;
     while ((p.route == kSmall ? 8u : 32u) << p.lanes_log2 < vocab) ++p.lanes_log2;
     const size_t per = 256u >> p.lanes_log2;
     p.blocks = (unsigned)std::min<size_t>((rows + per - 1) / per, kGroupBlocks);
-  } else if (rows < kSplitRows && vocab >= kSplitVocab) {
+  } else if (rows < kSplitRows && vocab > (loss ? kSplitLoss : kSplitStats)) {
     p.route = kSplit;
     p.chunks = (unsigned)((vocab + kSplitChunk - 1) / kSplitChunk);
   }
@@ -1013,9 +1016,11 @@ void launch_stats(const Plan &p, const PolicyArgs &a, Softmax *parts, float *pic
   else if (p.route == kSplit) {
     hipLaunchKernelGGL(policy_split_kernel<T>, dim3(rows * p.chunks), dim3(256), 0, s, a, p.chunks, parts, picked);
     hipLaunchKernelGGL(policy_join_kernel, dim3(rows), dim3(64), 0, s, a, p.chunks, (const Softmax *)parts, (const float *)picked);
-  } else if (a.vocab < kSplitChunk) hipLaunchKernelGGL((policy_stats_row_kernel<T, 1>), dim3(rows), dim3(256), 0, s, a);
-  else if (a.vocab < 2 * kSplitChunk) hipLaunchKernelGGL((policy_stats_row_kernel<T, 2>), dim3(rows), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((policy_stats_row_kernel<T, 4>), dim3(rows), dim3(256), 0, s, a);
+  } else if (a.vocab < kSplitChunk) hipLaunchKernelGGL((policy_stats_row_kernel<T, 256, 1>), dim3(rows), dim3(256), 0, s, a);
+  else if (a.vocab < 2 * kSplitChunk) hipLaunchKernelGGL((policy_stats_row_kernel<T, 256, 2>), dim3(rows), dim3(256), 0, s, a);
+  else if (rows < 256 && a.vocab <= 32768) hipLaunchKernelGGL((policy_stats_row_kernel<T, 1024, 4>), dim3(rows), dim3(1024), 0, s, a);
+  else if (rows < 256) hipLaunchKernelGGL((policy_stats_row_kernel<T, 1024, 8>), dim3(rows), dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((policy_stats_row_kernel<T, 256, 4>), dim3(rows), dim3(256), 0, s, a);
 }
 
 // Vectors a thread: the choice that keeps most rows in a CU at once, whose phases then overlap; of equal ones the smallest.
@@ -1092,8 +1097,8 @@ int ppo_xp_shape_logits_backward(int device, void *stream, int dtype, const void
   return shape("shape_logits_backward", device, stream, dtype, a, rows, vocab, rules, true);
 }
 
-size_t ppo_xp_policy_workspace(int dtype, size_t rows, size_t vocab, int loss) {
-  return rows && vocab ? plan_of(dtype, rows, vocab, loss != 0).bytes : 0;
+size_t ppo_xp_policy_workspace(size_t rows, size_t vocab, int loss) {
+  return rows && vocab ? plan_of(rows, vocab, loss != 0).bytes : 0;
 }
 
 int ppo_xp_action_stats(int device, void *stream, int dtype, const void *logits, int64_t logits_stride, const int64_t *actions,
@@ -1102,7 +1107,7 @@ int ppo_xp_action_stats(int device, void *stream, int dtype, const void *logits,
   if (rows == 0 || vocab == 0) return 0;
   if (!actions || !neglogps || !entropies) return ppoxp_fail(PPO_XP_EINVAL, "action_stats: NULL argument");
   if (rows > kMaxGrid) return ppoxp_fail(PPO_XP_EINVAL, "action_stats: %zu rows are too many for one launch", rows);
-  const Plan p = plan_of(dtype, rows, vocab, false);
+  const Plan p = plan_of(rows, vocab, false);
   if (int rc = check_workspace("action_stats", p, workspace, workspace_bytes)) return rc;
   PolicyArgs a{};
   a.logits = logits; a.stride = logits_stride; a.actions = actions; a.neglogps = neglogps; a.entropies = entropies;
@@ -1133,7 +1138,7 @@ int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, 
       !entropies || !stats)
     return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: NULL argument");
   if (rows > kMaxGrid) return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: %zu rows are too many for one launch", rows);
-  const Plan p = plan_of(dtype, rows, vocab, true);
+  const Plan p = plan_of(rows, vocab, true);
   if (int rc = check_workspace("policy_loss", p, workspace, workspace_bytes)) return rc;
   PolicyArgs a{};
   a.logits = logits; a.stride = logits_stride; a.actions = b->actions; a.neglogps = neglogps; a.entropies = entropies;

@@ -157,7 +157,7 @@ def action_stats(logits, actions):
     rows, vocab, stride = _matrix(logits, "action_stats")
     L, dt, d = _lib.load(), _DTYPES[logits.dtype], logits.get_device()
     ap = _vector(actions, rows, torch.int64, d, "actions")
-    n = L.ppo_xp_policy_workspace(dt, rows, vocab, 0)
+    n = L.ppo_xp_policy_workspace(rows, vocab, 0)
     ws = torch.empty(n, dtype=torch.uint8, device=logits.device) if n else None       # a new one each call: see policy_loss
     both = torch.empty(2, rows, dtype=torch.float32, device=logits.device)
     p = both.data_ptr()
@@ -190,7 +190,7 @@ def policy_loss(logits, values, batch, *, clip=0.2, ent_coef=0.01, vf_coef=0.5, 
     dlogits, dstride = _like(logits, out, "policy_loss")
     # one piece of memory for the workspace and the small results, from torch's allocator: calls on two streams and two captured
     # graphs never share it
-    n = -(-L.ppo_xp_policy_workspace(dt, rows, vocab, 1) // 4)
+    n = -(-L.ppo_xp_policy_workspace(rows, vocab, 1) // 4)
     buf = (torch.empty if rows and vocab else torch.zeros)(n + 3 * rows + 6, dtype=f32, device=logits.device)
     _, dvalues, neglogps, entropies, stats = buf.split((n, rows, rows, rows, 6))
     ws = buf.data_ptr()

@@ -68,17 +68,19 @@ def test_backward_refusals():
 
 
 def test_stats_and_loss_refusals():
-    need = L.ppo_xp_policy_workspace(0, 4, 100, 0)
-    st = lambda dtype=0, a=P, n=P, e=P, rows=4, ws=P, nb=1 << 40: L.ppo_xp_action_stats(0, None, dtype, P, 100, a, n, e, rows, 100, ws, nb)  # noqa: E731
+    need = L.ppo_xp_policy_workspace(4, 1 << 20, 0)
+    st = lambda dtype=0, a=P, n=P, e=P, rows=4, ws=P, nb=1 << 40: \
+        L.ppo_xp_action_stats(0, None, dtype, P, 1 << 20, a, n, e, rows, 1 << 20, ws, nb)  # noqa: E731
     refused(st(dtype=-1), "element type")
     refused(st(a=None), "NULL")
     refused(st(n=None), "NULL")
     refused(st(e=None), "NULL")
     refused(st(rows=1 << 31), "too many")
-    if need:
-        refused(st(ws=None), "workspace")
-        refused(st(nb=need - 1), "workspace")
-        refused(st(ws=P + 8), "workspace")
+    assert need > 0                                        # few rows of a million tokens are split over workgroups
+    refused(st(ws=None), "workspace")
+    refused(st(nb=need - 1), "workspace")
+    refused(st(ws=P + 8), "workspace")
+    assert L.ppo_xp_policy_workspace(4, 100, 0) == 0 and L.ppo_xp_policy_workspace(0, 100, 1) == 0
     assert st(rows=0) == 0
 
     def loss(batch=(P,) * 6, clip=0.2, ent=0.01, vf=0.5, denom=4.0, d=P, ds=100, dv=P, stats=P, ws=P, nb=1 << 40):
@@ -95,7 +97,7 @@ def test_stats_and_loss_refusals():
     refused(loss(ds=10), "apart")
     refused(loss(dv=None), "NULL")
     refused(loss(stats=None), "NULL")
-    need = L.ppo_xp_policy_workspace(0, 4, 100, 1)
+    need = L.ppo_xp_policy_workspace(4, 100, 1)
     assert need > 0
     refused(loss(ws=None), "workspace")
     refused(loss(nb=need - 1), "workspace")
