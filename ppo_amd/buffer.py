@@ -95,6 +95,7 @@ class ExperienceBuffer:
                               self.gamma, self.lam))
         self._L = L
         self.streaming = False
+        self.rows, self.rows_dtype = None, None   # new_quantized: the store of observation rows
 
     # -- constructors with the reference's names ------------------------------------------
     @classmethod
@@ -106,6 +107,39 @@ class ExperienceBuffer:
     def new_with_params(cls, num_envs, obs_size, capacity, gamma, lam, device=0):
         """ExperienceBuffer::new_with_params (buffer.rs:52-69)."""
         return cls(num_envs, obs_size, capacity, gamma, lam, device)
+
+    @classmethod
+    def new_quantized(cls, num_envs, row_size, capacity, format="int8", group=64, dtype=None, gamma=0.99, lam=0.95, device=0):
+        """A buffer whose observation rows (hidden states of `row_size` elements, f32 / bf16 / f16) are kept in 8 or 4 bits: quantised as
+        add_experience* writes them, read back as `dtype` (default f32) by the minibatches of a pass (quant.QuantizedRows).  The
+        other streams and the pass itself are the ordinary ones; rows are written and read on torch's current stream."""
+        import torch
+        from .quant import QuantizedRows
+        self = cls(num_envs, 1, capacity, gamma, lam, device)      # the handle's own rows: one unused float
+        self.rows = QuantizedRows(self.capacity * self.num_envs, row_size, format, group, device)
+        self.rows_dtype = torch.float32 if dtype is None else dtype
+        self._no_obs = torch.zeros(self.num_envs, 1, device=self.rows.codes.device)
+        return self
+
+    def _write_rows(self, obs, steps):
+        """Quantises the rows of `steps` steps that are about to be inserted at the ring's next places ([steps * N, row_size])."""
+        n, cap = self.num_envs, self.capacity
+        done, at = max(0, steps - cap), self.counter                # what a later step of this call overwrites is not written
+        while done < steps:
+            place = (at + done) % cap
+            run = min(steps - done, cap - place)
+            self.rows.write(obs[done * n:(done + run) * n], place * n)
+            done += run
+
+    def _device_rows(self, obs, steps):
+        import torch
+        t = torch.as_tensor(np.asarray(obs)) if not isinstance(obs, torch.Tensor) else obs
+        if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            t = t.to(torch.float32)
+        t = t.to(self.rows.codes.device)
+        if t.numel() != steps * self.num_envs * self.rows.row_size:
+            raise PpoXpPanic(_lib.EINVAL, f"add_experience: obs must be [NUM_ENVS, {self.rows.row_size}] a step (reference panics, buffer.rs:97-112)")
+        return t.reshape(steps * self.num_envs, self.rows.row_size)
 
     def close(self):
         if getattr(self, "_h", None) and self._h.value:
@@ -128,6 +162,8 @@ class ExperienceBuffer:
     # -- insert -----------------------------------------------------------------------------
     def add_experience(self, obs, rewards, actions, vals, dones, neglogps):
         """buffer.rs:84-121.  obs [NUM_ENVS, OBS_SIZE]; the rest [NUM_ENVS]; dones are bools."""
+        if self.rows is not None:
+            states, obs = self._device_rows(obs, 1), np.zeros((self.num_envs, 1), np.float32)
         obs = _np(obs, np.float32, "obs")
         rewards, vals, neglogps = (_np(x, np.float32, n) for x, n in ((rewards, "rewards"), (vals, "vals"), (neglogps, "neglogps")))
         actions = _np(actions, np.uint64, "actions")
@@ -138,11 +174,16 @@ class ExperienceBuffer:
         for name, a in (("rewards", rewards), ("actions", actions), ("vals", vals), ("dones", dones), ("neglogps", neglogps)):
             if a.ndim != 1 or a.shape[0] != self.num_envs or n != self.num_envs:
                 raise PpoXpPanic(_lib.EINVAL, f"add_experience: {name}/obs length != NUM_ENVS (reference panics, buffer.rs:97-112)")
+        if self.rows is not None:
+            self._write_rows(states, 1)
         p = lambda a: a.ctypes.data_as(C.c_void_p)
         check(self._L.ppo_xp_add(self._h, p(obs), p(rewards), p(actions), p(vals), p(dones), p(neglogps), n))
 
     def add_many(self, obs, rewards, actions, vals, dones, neglogps):
         """`steps` add_experience calls from [steps, N, ...] host arrays."""
+        if self.rows is not None:
+            steps = len(rewards)
+            states, obs = self._device_rows(obs, steps), np.zeros((steps, self.num_envs, 1), np.float32)
         obs = _np(obs, np.float32, "obs")
         rewards, vals, neglogps = (_np(x, np.float32, "") for x in (rewards, vals, neglogps))
         actions = _np(actions, np.uint64, "actions")
@@ -151,6 +192,8 @@ class ExperienceBuffer:
         if obs.shape != (steps, self.num_envs, self.obs_size) or any(
                 a.shape != (steps, self.num_envs) for a in (rewards, actions, vals, dones, neglogps)):
             raise PpoXpPanic(_lib.EINVAL, "add_many: shape mismatch")
+        if self.rows is not None:
+            self._write_rows(states, steps)
         p = lambda a: a.ctypes.data_as(C.c_void_p)
         check(self._L.ppo_xp_add_many(self._h, p(obs), p(rewards), p(actions), p(vals), p(dones), p(neglogps),
                                       self.num_envs, steps))
@@ -158,6 +201,10 @@ class ExperienceBuffer:
     def add_experience_device(self, obs, rewards, actions, vals, dones_f32, neglogps):
         """add_experience from torch CUDA tensors (f32 / i64 / f32 / f32 0-1 / f32), device to device."""
         import torch
+        if self.rows is not None:
+            if not obs.is_cuda or obs.dim() != 2 or obs.shape != (self.num_envs, self.rows.row_size):
+                raise PpoXpPanic(_lib.EINVAL, f"add_experience_device: CUDA rows [NUM_ENVS, {self.rows.row_size}] expected")
+            states, obs = obs, self._no_obs
         ts = [obs, rewards, actions, vals, dones_f32, neglogps]
         want = [torch.float32, torch.float32, torch.int64, torch.float32, torch.float32, torch.float32]
         for t, w in zip(ts, want):
@@ -169,6 +216,8 @@ class ExperienceBuffer:
         # current stream) and order torch's stream after them, so that neither an in-place update of the
         # source tensors by the next simulator step nor the caching allocator recycling a temporary can
         # race with a pending copy (no host synchronisation either way)
+        if self.rows is not None:
+            self._write_rows(states, 1)
         cur, hs = self._order_streams()
         if hs is not None:
             hs.wait_stream(cur)
@@ -213,12 +262,17 @@ class ExperienceBuffer:
 
     def training_views(self):
         """buffer.rs:142-175 → (observations [M, D], actions [M] i64, values [M], neglogps [M]):
-        zero-copy torch views of device memory, storage order."""
+        zero-copy torch views of device memory, storage order (quantised rows: a copy)."""
         import torch
         v = self._views()
         M, D, d = v.num_steps, self.obs_size, self.device
         self.sync()
-        return (device_tensor(v.observations, (M, D), torch.float32, d, self),
+        if self.rows is not None:
+            obs = self.rows.read(slice(0, M), dtype=self.rows_dtype)     # a copy: the rows as they read back
+            obs._ppo_owner = self
+        else:
+            obs = device_tensor(v.observations, (M, D), torch.float32, d, self)
+        return (obs,
                 device_tensor(v.actions, (M,), torch.int64, d, self),
                 device_tensor(v.values, (M,), torch.float32, d, self),
                 device_tensor(v.neglogps, (M,), torch.float32, d, self))
@@ -263,6 +317,8 @@ class ExperienceBuffer:
         """Device view of one raw stream in storage order over rows 0..len ('rewards', 'dones', ...)."""
         import torch
         v = self._views()
+        if name == "observations" and self.rows is not None:
+            return self.rows.read(slice(0, v.num_steps), dtype=self.rows_dtype)
         dt = torch.int64 if name == "actions" else torch.float32
         shape = (v.num_steps, self.obs_size) if name == "observations" else (v.num_steps,)
         self.sync()

@@ -132,6 +132,11 @@ class ExperienceBatcherIterator:
             if hs is not None:
                 cur.wait_stream(hs)
             buf._pass_perm = None
+        if buf.rows is not None:
+            # reads of quantised rows on torch's stream may still be using the previous pass's permutation
+            cur, hs = buf._order_streams()
+            if hs is not None:
+                hs.wait_stream(cur)
         if perm is not None and hasattr(perm, "is_cuda") and perm.is_cuda:
             import torch
             if perm.numel() != len(batcher) or perm.dtype not in (torch.int32,) or not perm.is_contiguous():
@@ -191,10 +196,27 @@ class ExperienceBatcherIterator:
             buf.sync()
         B, D, d = v.batch_size, v.obs_size, buf.device
         f32, i64 = torch.float32, torch.int64
+        obs = device_tensor(v.observations, (B, D), f32, d, buf) if buf.rows is None else self._read_rows(v.index, B)
         return ExperienceBatch(
-            device_tensor(v.observations, (B, D), f32, d, buf), device_tensor(v.actions, (B,), i64, d, buf),
+            obs, device_tensor(v.actions, (B,), i64, d, buf),
             device_tensor(v.values, (B,), f32, d, buf), device_tensor(v.neglogps, (B,), f32, d, buf),
             device_tensor(v.returns, (B,), f32, d, buf), device_tensor(v.advantages, (B,), f32, d, buf))
+
+    def _read_rows(self, k, B):
+        """Minibatch k's observation rows out of the buffer's quantised store, by the pass's own permutation and window
+        (data.rs:121-126), as a new tensor on torch's current stream."""
+        import torch
+        buf, L = self.batcher.buffer, self.batcher._L
+        M = len(self.batcher)
+        ptr = L.ppo_xp_pass_perm_device(buf.handle)      # a keyed bijection is written out on the handle's stream the first time
+        if not ptr:
+            check(_lib.ESTATE)
+        cur, hs = buf._order_streams()
+        if hs is not None:
+            cur.wait_stream(hs)
+        start = min(k * B, M - B)
+        index = device_tensor(ptr, (M,), torch.uint32, buf.device, buf)[start:start + B]
+        return buf.rows.read(index, dtype=buf.rows_dtype)
 
     def next_host(self, out: "HostBatch | None" = None) -> "HostBatch | None":
         """Iterator::next as the reference's caller sees it (data.rs:166-182 feeds six host Vecs to
@@ -202,6 +224,7 @@ class ExperienceBatcherIterator:
         HostBatch.pinned).  Returns None when the pass is exhausted.  With out=None every call fills the SAME page-locked
         set owned by the iterator: copy what must outlive the next call."""
         buf = self.batcher.buffer
+        self._no_quantized_rows()
         if out is None:      # one page-locked set per iterator, reused by every call (a fresh hipHostMalloc per minibatch costs more than the copy)
             if getattr(self, "_host_batch", None) is None:
                 self._host_batch = HostBatch.pinned(self.batcher.batch_size, buf.obs_size)
@@ -216,6 +239,7 @@ class ExperienceBatcherIterator:
         (ppo_xp_pass_next_host_pipelined): two page-locked slots alternate, so a yielded batch is valid until the one
         after next is asked for.  `slots`: two HostBatch objects (default: a page-locked pair owned by the iterator)."""
         buf = self.batcher.buffer
+        self._no_quantized_rows()
         if slots is None:
             if getattr(self, "_host_pair", None) is None:
                 self._host_pair = (HostBatch.pinned(self.batcher.batch_size, buf.obs_size),
@@ -233,6 +257,10 @@ class ExperienceBatcherIterator:
                 return
             yield a.view(a._c.batch_size, a._c.index)
             a, b = b, a
+
+    def _no_quantized_rows(self):
+        if self.batcher.buffer.rows is not None:
+            raise PpoXpPanic(_lib.EINVAL, "host minibatches: the rows of this buffer are quantised on the device; iterate over device minibatches")
 
     def perm(self) -> np.ndarray:
         """The permutation of this pass (host copy)."""
