@@ -18,7 +18,7 @@ def half(dtype):
 
 
 def floor_of(dtype):       # half of the least subnormal: what a rounding near zero can be off by
-    return {torch.float64: 0.0, F32: 0.0, BF16: 2.0 ** -134, F16: 2.0 ** -25}[dtype]
+    return {torch.float64: 0.0, F32: 2.0 ** -150, BF16: 2.0 ** -134, F16: 2.0 ** -25}[dtype]
 
 
 def gen(seed):
@@ -278,7 +278,9 @@ def softmax64(logits, actions):
     adds = (V / 64 + 48) * U
     rel_s = 3 * U * (-ts) + 2 * U + adds
     err_ts = 3 * U * (p * dz * dz).sum(1) + (2 * U + adds + rel_s) * (-ts) + 2 * U * (-ts)
-    err_nlp = rel_s + 2 * U * (lns.abs() + d_a.abs().clamp(max=1e30) + nlp.abs().clamp(max=1e30))
+    # log2 s, the action's power of two, their difference and the factor ln 2: 2 u each way of what they are (an action that is
+    # forbidden has neither)
+    err_nlp = rel_s + 2 * U * (lns.abs() + torch.where(torch.isfinite(d_a), d_a.abs() + nlp.abs(), 0.0))
     err_ent = rel_s + err_ts + 2 * U * (lns.abs() + ts.abs() + ent.abs())
     return dict(m=m, d=d, p=p, lns=lns, ts=ts, nlp=nlp, ent=ent, rel_s=rel_s, err_ts=err_ts, err_nlp=err_nlp, err_ent=err_ent)
 
@@ -396,6 +398,11 @@ def loss64(logits, b, a, clip, ent_c, vf_c, n):
     size = w["p"] * (gain.abs()[:, None] + ent_c * (lnp.abs() + w["ent"].abs()[:, None] + dist + w["ts"].abs()[:, None])) / n
     tol = size * ((3 * dist + 24) * U + 2 * w["rel_s"][:, None]) + w["p"] * ent_c * w["err_ts"][:, None] / n \
         + (rel_g * gain.abs() / n)[:, None] * (w["p"] + hit)
+    # where ln p + H cancels: x = l log2(e) - m2 is relative to a rounded m2 = m log2(e), off by at most u |m2|; that shift is taken
+    # out of the constant term again, which rounds three times numbers of its size
+    tol = tol + 4 * U * U * torch.where(torch.isfinite(w["m"]), w["m"].abs().clamp(max=4096.0), 0.0) * w["p"] * ent_c / n
+    # a power of two below 2^-126 is returned as 0 by the hardware's exponential: off by less than 2^-126 times its factor
+    tol = tol + 2.0 ** -126 * (gain.abs()[:, None] + ent_c * (lnp.abs() + w["ent"].abs()[:, None] + dist)) / n
     tol = tol + half(logits.dtype) * (d.abs() + tol) + floor_of(logits.dtype)
     keep = lambda t: torch.where(real, t, 0.0)  # noqa: E731
     terms = [keep(pg), keep(torch.maximum(q1, q2) / 2), keep(w["ent"]), keep((w["nlp"] - old) ** 2 / 2), keep(((ratio - 1).abs() > clip).double())]
