@@ -127,6 +127,7 @@ SYMBOLS = {
 }
 
 _lib = None
+_torchcall = None
 
 
 def _share_hip_runtime_with_torch():
@@ -166,6 +167,23 @@ def load() -> C.CDLL:
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+def torchcall():
+    """The compiled step from torch tensors to the C ABI (csrc/torchcall.cpp) that policy.py and quant.py call, bound to load()'s library."""
+    global _torchcall
+    if _torchcall is None:
+        import torch
+        L = load()
+        try:
+            from . import _torchcall as T
+        except ImportError as e:
+            raise PpoXpError(ENODEV, f"ppo_amd/_torchcall.so is not built for this torch (run `make -C ppo_amd/csrc`): {e}") from e
+        names = ("shape_logits", "shape_logits_backward", "action_stats", "policy_workspace", "policy_loss", "quantize_rows", "dequantize_rows")
+        stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+        T.setup(PpoXpPanic, check, stream, tuple(C.cast(getattr(L, "ppo_xp_" + n), _vp).value for n in names))
+        _torchcall = T
+    return _torchcall
 
 
 def last_error() -> str:

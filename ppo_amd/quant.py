@@ -7,11 +7,17 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import check
-from .policy import _DTYPES, _matrix, _panic, _raw_stream
+from ._lib import EINVAL, PpoXpPanic
+
+_call = _lib.torchcall()                          # csrc/torchcall.cpp
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 #: format -> (PPO_XP_Q_*, type of the codes)
 FORMATS = {"int8": (1, torch.int8), "e4m3": (2, torch.float8_e4m3fn), "int4": (3, torch.uint8)}
+
+
+def _panic(msg):
+    raise PpoXpPanic(EINVAL, msg)
 
 
 class QuantizedRows:
@@ -50,7 +56,6 @@ class QuantizedRows:
             if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
                 _panic("QuantizedRows: rows of codes and scales must be contiguous and must not overlap")
         self.codes, self.scales, self.row_size, self.format, self.group = codes, scales, int(row_size), format, int(group)
-        self._store = (codes.data_ptr(), max(codes.stride(0), nbytes), scales.data_ptr(), max(scales.stride(0), scales.shape[1]))
         self._kind = kind
 
     def __len__(self):
@@ -58,36 +63,16 @@ class QuantizedRows:
 
     def write(self, rows, at: int = 0):
         """Quantises `rows` [n, row_size] (f32, bf16, f16) into rows at .. at + n of the store."""
-        n, width, stride = _matrix(rows, "write")
-        dev = self.codes.device
-        if width != self.row_size or rows.device != dev or at < 0:
-            _panic(f"write: rows of {self.row_size} on {dev} and at >= 0 expected")
-        cp, cs, sp, ss = self._store
-        check(_lib.load().ppo_xp_quantize_rows(dev.index, _raw_stream(dev.index), _DTYPES[rows.dtype], rows.data_ptr(), stride, n, width, self._kind,
-                                               self.group, cp, cs, sp, ss, self.codes.shape[0], at))
+        _call.write(self.codes, self.scales, self.row_size, self._kind, self.group, rows, at)
 
     def read(self, index=None, dtype=torch.float32, out=None):
         """Rows index[j] (contiguous int32 / int64 CUDA tensor), a slice of rows, or all rows, as `dtype`."""
-        dev, store = self.codes.device, self.codes.shape[0]
         if dtype not in _DTYPES:
             _panic("read: f32, bf16 or f16 expected")
-        ip = bits = at = 0
+        at = n = 0
         if index is None or isinstance(index, slice):
-            at, end, step = (index or slice(None)).indices(store)
+            at, end, step = (index or slice(None)).indices(len(self))
             if step != 1:
                 _panic("read: a slice of consecutive rows expected")
-            n = max(0, end - at)
-        else:
-            if index.dtype not in (torch.int32, torch.int64) or index.device != dev or index.dim() != 1 or not index.is_contiguous():
-                _panic("read: a contiguous int32 or int64 index on the store's device expected")
-            n, ip, bits = index.shape[0], index.data_ptr(), 32 if index.dtype is torch.int32 else 64
-        if out is None:
-            out, ostride = torch.empty(n, self.row_size, dtype=dtype, device=dev), self.row_size
-        else:
-            if out.dtype is not dtype or out.device != dev or out.shape != (n, self.row_size):
-                _panic(f"read: out must be {dtype} [{n}, {self.row_size}] on {dev}")
-            ostride = _matrix(out, "read")[2]
-        cp, cs, sp, ss = self._store
-        check(_lib.load().ppo_xp_dequantize_rows(dev.index, _raw_stream(dev.index), _DTYPES[dtype], cp, cs, sp, ss, store, self.row_size, self._kind,
-                                                 self.group, ip or None, bits, at, n, out.data_ptr(), ostride))
-        return out
+            index, n = None, max(0, end - at)
+        return _call.read(self.codes, self.scales, self.row_size, self._kind, self.group, index, at, n, _DTYPES[dtype], out)

@@ -6,9 +6,10 @@ import pytest
 import torch
 
 import ppo_amd
-from ppo_amd import _lib, policy
+from ppo_amd import _lib
 
 L = _lib.load()
+RULES = struct.Struct("19q4f2i")                  # ppo_xp_logit_rules
 P = 0x10000            # an address nothing looks at: every call below is refused first
 
 
@@ -18,7 +19,7 @@ def rules(**kw):
              mask_rows=0, mask_row=0, repetition=1.0, presence=0.0, frequency=0.0, temperature=1.0, history_bits=64, mask_kind=0)
     assert set(kw) <= set(d)
     d.update(kw)
-    return policy._RULES.pack(*d.values())
+    return RULES.pack(*d.values())
 
 
 def shape(dtype=0, logits=P, ls=100, out=P, os_=100, rows=4, vocab=100, r=None):
