@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "ops_common.h"
 
@@ -21,19 +22,20 @@ struct ShapeArgs {
   void *out;
   int64_t in_stride, logits_stride, out_stride;
   size_t rows;
-  unsigned vocab, chunks;                       // chunks of a row, where a row fills a workgroup
+  unsigned vocab, chunks, part;                 // chunks of a row and their elements, where a row fills a workgroup
   unsigned rows_per, units, magic, scan_log2;   // else rows of a workgroup, 8-element units of a row, 2^20 / units, lanes that scan a row
   ppo_xp_logit_rules r;
 };
 
 enum ShapeMode { kForward, kGather, kReadAll };
-constexpr int kShapeVecs = 4;                        // 8-element vectors a thread
-constexpr unsigned kShapeChunk = 256 * 8 * kShapeVecs;
+// Elements of a workgroup, with VECS vectors of 8 a thread.
+constexpr unsigned shape_chunk(int vecs) { return 256 * 8 * vecs; }
 constexpr unsigned kPromptOnly = 0x80000000u;        // table word: occurrences in the generated part, this bit: in the rest
 
 // Where element e of a workgroup's chunk has its table word: the lower and the upper halves of the vectors lie apart, so that a
 // wave reads each half without bank conflicts.
-__device__ __forceinline__ unsigned table_slot(unsigned e) { return ((e & 4) ? kShapeChunk / 2 : 0) + (e >> 3) * 4 + (e & 3); }
+template <int VECS>
+__device__ __forceinline__ unsigned table_slot(unsigned e) { return ((e & 4) ? shape_chunk(VECS) / 2 : 0) + (e >> 3) * 4 + (e & 3); }
 
 struct RowRules {
   float rep, inv_rep, pres, freq, inv_t;
@@ -79,21 +81,23 @@ __device__ __forceinline__ unsigned allowed8(const RowRules &q, int kind, unsign
 // (kGather), or only that it was seen, where all logits are read (kReadAll).
 // Every workgroup of a row reads the row's whole history; that is cheaper than sorting it while the history is shorter than the
 // vocabulary.  Elements then take their word without a branch: at a seen token in a hundred a wave would enter it anyway.
-template <typename T, bool HIST, int MODE, bool MULTI>
+template <typename T, bool HIST, int MODE, bool MULTI, int VECS>
 __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
   constexpr bool BACKWARD = MODE != kForward;
-  __shared__ __attribute__((aligned(16))) unsigned table[HIST ? kShapeChunk : 4];
+  constexpr unsigned CHUNK = shape_chunk(VECS);
+  __shared__ __attribute__((aligned(16))) unsigned table[HIST ? CHUNK : 4];
   const ppo_xp_logit_rules &r = a.r;
   const unsigned tid = threadIdx.x;
   const size_t row0 = MULTI ? (size_t)blockIdx.x * a.rows_per : blockIdx.x / a.chunks;
-  const unsigned c0 = MULTI ? 0 : (blockIdx.x % a.chunks) * kShapeChunk;
+  const unsigned c0 = MULTI ? 0 : (blockIdx.x % a.chunks) * a.part;
   const unsigned here = MULTI ? (unsigned)min((size_t)a.rows_per, a.rows - row0) : 1;    // rows of this workgroup
+  const unsigned c1 = MULTI ? a.vocab : min(a.vocab, c0 + a.part);
   RowRules one;
   if (!MULTI) one = row_rules(r, row0);
   // unit k of this thread: its row and first element, and whether there is one
   auto place = [&](int k, size_t &row, unsigned &e) {
     const unsigned u = k * 256 + tid;
-    if (!MULTI) { row = row0; e = c0 + u * 8; return e < a.vocab; }
+    if (!MULTI) { row = row0; e = c0 + u * 8; return e < c1; }
     const unsigned rl = (u * a.magic) >> 20;
     row = row0 + rl;
     e = (u - rl * a.units) * 8;
@@ -102,13 +106,13 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
 
   auto fetch = [&](Raw8<T> *to, const void *from, int64_t stride) {
 #pragma unroll
-    for (int k = 0; k < kShapeVecs; ++k) {
+    for (int k = 0; k < VECS; ++k) {
       size_t row; unsigned e;
-      const bool live = place(k, row, e);
-      if (live && e + 8 <= a.vocab) {
-        to[k].load((const T *)from + (int64_t)row * stride + e);
-      } else {                                       // a row's end, or nothing: clamped addresses, no further branch
-        const T *p = (const T *)from + (int64_t)(live ? row : row0) * stride;
+      if (!place(k, row, e)) { row = row0; e = 0; }   // nothing here: the whole wave stays on the wide load
+      const T *p = (const T *)from + (int64_t)row * stride;
+      if (e + 8 <= a.vocab) {
+        to[k].load(p + e);
+      } else {                                       // a row's end: clamped addresses, no further branch
         T q[8];
         float y[8];
 #pragma unroll
@@ -119,20 +123,20 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
       }
     }
   };
-  Raw8<T> raw[kShapeVecs], own[MODE == kReadAll ? kShapeVecs : 1];
+  Raw8<T> raw[VECS], own[MODE == kReadAll ? VECS : 1];
   fetch(raw, a.in, a.in_stride);
   if (MODE == kReadAll) fetch(own, a.logits, a.logits_stride);
-  unsigned ok[kShapeVecs];                           // with one row a workgroup the mask's bits are on their way as well
+  unsigned ok[VECS];                           // with one row a workgroup the mask's bits are on their way as well
   if (!MULTI) {
 #pragma unroll
-    for (int k = 0; k < kShapeVecs; ++k) {
+    for (int k = 0; k < VECS; ++k) {
       const unsigned e = c0 + (k * 256 + tid) * 8;
       ok[k] = one.mask && r.mask_kind == PPO_XP_MASK_BITS ? one.mask[min(e, a.vocab - 1) / 8] : 0xffu;
     }
   }
   if (HIST) {
 #pragma unroll
-    for (int k = 0; k < kShapeVecs; ++k) {
+    for (int k = 0; k < VECS; ++k) {
       unsigned word = 0;
       if (MODE == kGather) {
         float inv_t = one.inv_t;
@@ -144,7 +148,7 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
         word = __builtin_bit_cast(unsigned, inv_t);
       }
       *(u32x4 *)(table + (k * 256 + tid) * 4) = u32x4(word);
-      *(u32x4 *)(table + kShapeChunk / 2 + (k * 256 + tid) * 4) = u32x4(word);
+      *(u32x4 *)(table + CHUNK / 2 + (k * 256 + tid) * 4) = u32x4(word);
     }
     __syncthreads();
     const unsigned lanes = MULTI ? 1u << a.scan_log2 : 256u;
@@ -174,14 +178,14 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
         float l[kTokens];
 #pragma unroll
         for (int j = 0; j < kTokens; ++j) {
-          const bool in_chunk = tok[j] >= c0 && tok[j] < (int64_t)min(a.vocab, c0 + kShapeChunk) && k0 + j * lanes < end;
+          const bool in_chunk = tok[j] >= c0 && tok[j] < (int64_t)c1 && k0 + j * lanes < end;
           if (!in_chunk) tok[j] = -1;
           if (MODE == kGather) l[j] = in_chunk ? (float)logits[tok[j]] : 0.f;
         }
 #pragma unroll
         for (int j = 0; j < kTokens; ++j) {
           if (tok[j] < 0) continue;
-          unsigned *word = table + table_slot((unsigned)tok[j] - c0 + rl * a.units * 8);
+          unsigned *word = table + table_slot<VECS>((unsigned)tok[j] - c0 + rl * a.units * 8);
           if (MODE == kGather) *word = __builtin_bit_cast(unsigned, l[j] > 0.f ? up : down);   // the same from every occurrence
           else if (MODE == kReadAll) *word = 1;
           else if (k0 + j * lanes >= gen) atomicAdd(word, 1u);
@@ -192,7 +196,7 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
     __syncthreads();
   }
 #pragma unroll
-  for (int k = 0; k < kShapeVecs; ++k) {
+  for (int k = 0; k < VECS; ++k) {
     size_t row; unsigned e;
     if (!place(k, row, e)) continue;
     const RowRules q = MULTI ? row_rules(r, row) : one;
@@ -200,7 +204,7 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
     u32x4 c[2] = {u32x4(0), u32x4(0)};
     if (HIST) {
       c[0] = *(const u32x4 *)(table + (k * 256 + tid) * 4);
-      c[1] = *(const u32x4 *)(table + kShapeChunk / 2 + (k * 256 + tid) * 4);
+      c[1] = *(const u32x4 *)(table + CHUNK / 2 + (k * 256 + tid) * 4);
     }
     float x[8];
 #pragma unroll
@@ -910,18 +914,21 @@ int check_rules(const char *who, const ppo_xp_logit_rules *r, size_t rows, size_
 }
 
 template <typename T, bool HIST, int MODE>
-void launch_shape(const ShapeArgs &a, dim3 grid, hipStream_t s) {
-  if (a.rows_per > 1) hipLaunchKernelGGL((shape_logits_kernel<T, HIST, MODE, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((shape_logits_kernel<T, HIST, MODE, false>), grid, dim3(256), 0, s, a);
+void launch_shape(const ShapeArgs &a, dim3 grid, bool narrow, hipStream_t s) {
+  constexpr int WIDE = std::is_same<T, float>::value && !HIST ? 1 : 4;       // never wide: see shape()
+  if (narrow && a.rows_per > 1) hipLaunchKernelGGL((shape_logits_kernel<T, HIST, MODE, true, 1>), grid, dim3(256), 0, s, a);
+  else if (narrow) hipLaunchKernelGGL((shape_logits_kernel<T, HIST, MODE, false, 1>), grid, dim3(256), 0, s, a);
+  else if (a.rows_per > 1) hipLaunchKernelGGL((shape_logits_kernel<T, HIST, MODE, true, WIDE>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((shape_logits_kernel<T, HIST, MODE, false, WIDE>), grid, dim3(256), 0, s, a);
 }
 template <typename T>
-void launch_shape(const ShapeArgs &a, dim3 grid, hipStream_t s, bool hist, bool backward) {
-  if (!backward) hist ? launch_shape<T, true, kForward>(a, grid, s) : launch_shape<T, false, kForward>(a, grid, s);
-  else if (!hist) launch_shape<T, false, kGather>(a, grid, s);
+void launch_shape(const ShapeArgs &a, dim3 grid, bool narrow, hipStream_t s, bool hist, bool backward) {
+  if (!backward) hist ? launch_shape<T, true, kForward>(a, grid, narrow, s) : launch_shape<T, false, kForward>(a, grid, narrow, s);
+  else if (!hist) launch_shape<T, false, kGather>(a, grid, narrow, s);
   // Fetching the logits of seen tokens one by one costs as much as reading them all at about a token in 50 (2048 x 50001 bf16, us one
   // by one against all: 133 and 132 at 1024 tokens a row, 164 and 134 at 2048, 232 and 157 at 4096); histories may be partly filled.
-  else if ((uint64_t)a.r.hist_len * 32 < a.vocab) launch_shape<T, true, kGather>(a, grid, s);
-  else launch_shape<T, true, kReadAll>(a, grid, s);
+  else if ((uint64_t)a.r.hist_len * 32 < a.vocab) launch_shape<T, true, kGather>(a, grid, narrow, s);
+  else launch_shape<T, true, kReadAll>(a, grid, narrow, s);
 }
 
 int shape(const char *who, int device, void *stream, int dtype, ShapeArgs &a, size_t rows, size_t vocab, const ppo_xp_logit_rules *rules,
@@ -930,23 +937,34 @@ int shape(const char *who, int device, void *stream, int dtype, ShapeArgs &a, si
   if (rows == 0 || vocab == 0) return 0;
   a.rows = rows;
   a.vocab = (unsigned)vocab;
-  a.chunks = (unsigned)((vocab + kShapeChunk - 1) / kShapeChunk);
-  // rows that fill less than half a workgroup's part share one (one workgroup a row: 113 us at 262144 x 32 bf16)
   a.units = (unsigned)((vocab + 7) / 8);
-  a.rows_per = (unsigned)std::min<size_t>(kShapeChunk / 8 / std::min(a.units, kShapeChunk / 8), rows);
+  const bool hist = rules->history && rules->hist_rows > 0 && rules->hist_len > 0;
+  // A workgroup's part is 8192 elements, or 2048 where a row is no longer than that, where 8192 leave CUs idle, and for f32 without a
+  // history, whose wider elements fill a wave's loads by themselves.  In us a call, parts of 8192 | 2048: f32 without a history
+  // 4096 x 151 8.2 | 4.1, 16384 x 4000 102 | 96, 2048 x 50001 158 | 149; bf16 with a history of 1024 tokens 4096 x 151 13.8 | 6.6,
+  // 65536 x 1000 143 | 134, 8 x 131072 5.8 | 4.3, 64 x 32768 (256 workgroups of 8192) 6.0 | 5.3, 32 x 131072 (512) 6.7 | 7.8,
+  // 16384 x 4000 80 | 91, 1024 x 131072 117 | 168.
+  const unsigned long_chunks = (a.units + shape_chunk(4) / 8 - 1) / (shape_chunk(4) / 8);
+  const bool narrow = a.units <= shape_chunk(1) / 8 || (dtype == PPO_XP_F32 && !hist) || rows * long_chunks <= 256;
+  const unsigned part = shape_chunk(narrow ? 1 : 4) / 8;
+  a.chunks = (a.units + part - 1) / part;
+  // rows that fill less than half a workgroup's part share one (one workgroup a row: 113 us at 262144 x 32 bf16)
+  a.rows_per = (unsigned)std::min<size_t>(part / std::min(a.units, part), rows);
+  // workgroups go to the 8 XCDs in turn, and of an even number of chunks a short last one is always the same XCDs': equal parts then
+  // (4096 x 10000 f32 with a history, 8192 and 1808: 91 us, 5056 and 4944: 71; with an odd number they cost 2048 x 50001 bf16 16 %)
+  a.part = a.chunks % 2 ? part * 8 : ((a.units + a.chunks - 1) / a.chunks + 7) / 8 * 64;
+  if (rows > kMaxGrid / a.chunks) return ppoxp_fail(PPO_XP_EINVAL, "%s: %zu rows of %zu are too many for one launch", who, rows, vocab);
   a.magic = ((1u << 20) + a.units - 1) / a.units;
   a.scan_log2 = 8;
   while (a.scan_log2 && (256u >> a.scan_log2) < a.rows_per) --a.scan_log2;
   a.r = *rules;
-  if (rows > kMaxGrid / a.chunks) return ppoxp_fail(PPO_XP_EINVAL, "%s: %zu rows of %zu are too many for one launch", who, rows, vocab);
   DeviceGuard dev(device, who);
   if (dev.rc()) return dev.rc();
   const dim3 grid((unsigned)(a.rows_per > 1 ? (rows + a.rows_per - 1) / a.rows_per : rows * a.chunks));
-  const bool hist = rules->history && rules->hist_rows > 0 && rules->hist_len > 0;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == PPO_XP_F32) launch_shape<float>(a, grid, s, hist, backward);
-  else if (dtype == PPO_XP_BF16) launch_shape<__bf16>(a, grid, s, hist, backward);
-  else launch_shape<_Float16>(a, grid, s, hist, backward);
+  if (dtype == PPO_XP_F32) launch_shape<float>(a, grid, narrow, s, hist, backward);
+  else if (dtype == PPO_XP_BF16) launch_shape<__bf16>(a, grid, narrow, s, hist, backward);
+  else launch_shape<_Float16>(a, grid, narrow, s, hist, backward);
   return launched(who);
 }
 

@@ -146,7 +146,10 @@ def make_rules(g, R, V, L, mask, bias, layout, per_row=True, tokens=torch.int64)
 SHAPES = [(1, 1, 0, "none", "none", "rows"), (1, 2, 1, "bits", "none", "rows"), (3, 7, 5, "bytes", "shared", "time"),
           (5, 8, 17, "bits", "row", "rows_of_others"), (9, 31, 40, "bytes_picked", "none", "apart"), (4, 33, 0, "bits", "shared", "rows"),
           (6, 151, 300, "bits_picked", "row", "time"), (2, 2047, 64, "shared", "none", "rows"), (3, 8192, 700, "bits", "shared", "rows"),
-          (2, 8193, 1000, "bytes", "row", "time"), (2, 20011, 513, "bits", "none", "rows_of_others"), (67, 129, 33, "bytes", "shared", "apart")]
+          (2, 8193, 1000, "bytes", "row", "time"), (2, 20011, 513, "bits", "none", "rows_of_others"), (67, 129, 33, "bytes", "shared", "apart"),
+          # enough rows for the workgroups with longer parts: several chunks, several rows a workgroup, short and long histories
+          (90, 20011, 40, "bits", "shared", "rows"), (261, 4095, 33, "bytes", "none", "time"), (300, 3001, 120, "bits_picked", "none", "apart"),
+          (262, 5000, 160, "bits", "row", "rows_of_others"), (257, 8200, 0, "bytes_picked", "shared", "rows"), (40, 2048, 9, "bits", "none", "rows")]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
