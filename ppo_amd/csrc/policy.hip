@@ -979,11 +979,12 @@ struct Plan {
   size_t o_slices = 0, o_ticket = 0, o_parts = 0, o_picked = 0, bytes = 0;
 };
 
-// Few long rows leave most of the 256 CUs idle with a workgroup each; the split costs a launch more (4 us of the host's time) and a
-// second read out of the caches.  Measured in us a call, one workgroup a row | split: statistics of 8 x 131072 f32 9.0 | 12.5,
-// 8 x 262144 f32 16.4 | 12.5, 200 x 262144 f32 32.4 | 33.7; objective of 8 x 65536 bf16 17.5 | 20.3, 8 x 131072 f32 27.4 | 20.2,
-// 200 x 131072 bf16 26.0 | 33.5.
-constexpr size_t kSplitRows = 128, kSplitLoss = 65536, kSplitStats = 131072;   // rows, tokens
+// Few long rows leave most of the 256 CUs idle with a workgroup each; the split costs a launch more (2 us of the host's time, which
+// bounds all of these up to 32 rows) and a second read out of the caches.  Measured in us a call, one workgroup a row | split:
+// statistics of 8 x 65536 f32 6.2 | 8.3, bf16 6.7 | 8.4, 8 x 131072 f32 8.9 | 8.3, bf16 10.6 | 8.1, 100 x 131072 f32 13.4 | 12.4,
+// 128 x 131072 bf16 11.9 | 11.8; objective of 8 x 50001 f32 11.6 | 12.4, bf16 13.0 | 12.2, 8 x 131072 f32 27.6 | 12.5,
+// 100 x 131072 bf16 22.0 | 20.1, 128 x 131072 bf16 22.8 | 23.7.
+constexpr size_t kSplitRows = 128, kSplitLoss = 65536, kSplitStats = 98304;   // rows, tokens
 
 Plan plan_of(size_t rows, size_t vocab, bool loss) {
   Plan p;

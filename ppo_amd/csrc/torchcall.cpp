@@ -213,6 +213,14 @@ PyObject *shape_backward(PyObject *const *a) {              // grad, logits, rul
 
 at::TensorOptions floats(const at::Tensor &like) { return at::TensorOptions().dtype(at::kFloat).device(like.device()); }
 
+// Elements at .. at + n of a tensor just allocated, as a tensor of its own (narrow() makes a view, which costs 0.6 us more).
+PyObject *piece(const at::Tensor &of, int64_t at, int64_t n) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(of.storage()), of.key_set(), of.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(of.storage_offset() + at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return THPVariable_Wrap(t);
+}
+
 PyObject *stats(PyObject *const *a) {                       // logits, actions
   const at::Tensor &t = some(a[0], "action_stats");
   const Matrix l = matrix(t, "action_stats");
@@ -225,8 +233,8 @@ PyObject *stats(PyObject *const *a) {                       // logits, actions
   done(launch(g_stats, l.device, stream_of(l.device), l.dtype, l.p, l.stride, (const int64_t *)actions, p + ws, p + ws + l.rows, l.rows, l.cols, p, ws * 4));
   PyObject *r = PyTuple_New(2);
   if (!r) throw Raised{};
-  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(buf.narrow(0, ws, l.rows)));
-  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(buf.narrow(0, ws + l.rows, l.rows)));
+  PyTuple_SET_ITEM(r, 0, piece(buf, ws, l.rows));
+  PyTuple_SET_ITEM(r, 1, piece(buf, ws + l.rows, l.rows));
   return r;
 }
 
@@ -265,9 +273,9 @@ PyObject *loss(PyObject *const *a) {                        // logits, values, b
               l.cols, p, ws * 4));
   PyObject *r = PyTuple_New(5);
   if (!r) throw Raised{};
-  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(buf.narrow(0, ws + 3 * n, 6)));
+  PyTuple_SET_ITEM(r, 0, piece(buf, ws + 3 * n, 6));
   PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(out));
-  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(r, 2 + i, THPVariable_Wrap(buf.narrow(0, ws + i * n, n)));
+  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(r, 2 + i, piece(buf, ws + i * n, n));
   return r;
 }
 
