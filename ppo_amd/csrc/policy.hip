@@ -575,39 +575,60 @@ __device__ __forceinline__ void put_block(const PolicyArgs &a, const double sum[
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
 }
 
-// Up to kSmallVocab tokens, the action sets of ordinary environments: lane i of a row's `lanes` lanes holds elements
-// i, i + lanes, ... as floats (SLOTS of them), with their powers kept for the gradient.  What a row costs beside its elements is
-// as much as 15 of them, so a row gets as few lanes as 8 elements each allow (10 each: 20.7 against 16.8 us at 262144 x 18 f32, since
-// one access of the wave then touches twice the lines).
+// Up to kSmallVocab tokens, the action sets of ordinary environments: a lane a row, since what a row costs beside its elements is as
+// much as 15 of them.  A wave's 64 rows come in and leave as one run of elements, 64 neighbours an access, and are turned in shared
+// memory, where rows lie an odd number of floats apart, free of bank conflicts.  SLOTS elements a lane, a multiple of 4, the last 3
+// perhaps beyond the row.  Memory bounds it: the objective of 1048576 x 32 f32 moves 306 MB in 60 us; with several lanes a row and no
+// turning it took 120 us, 262144 x 18 f32 18.9 us against 16.2 us, statistics of 262144 x 32 f32 7.9 against 9.2 us.
 constexpr unsigned kSmallVocab = 32, kGroupBlocks = 1536;
 
+__device__ __forceinline__ void wave_lds_fence() {            // what the wave's lanes wrote to LDS, its other lanes read afterwards
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <typename T, bool LOSS, int SLOTS>
-__global__ __launch_bounds__(256) void policy_small_kernel(PolicyArgs a, unsigned lanes_log2) {
+__global__ __launch_bounds__(256, 4) void policy_small_kernel(PolicyArgs a, unsigned magic) {   // magic: 2^16 / vocab, rounded up
   __shared__ double red[4][5];
-  const unsigned lanes = 1u << lanes_log2, sub = threadIdx.x & (lanes - 1);
-  const size_t per_block = 256u >> lanes_log2;
+  __shared__ float turn[4][64 * (SLOTS + 1)];
+  const unsigned vocab = a.vocab, even = vocab % 2 ? 0 : magic;
+  unsigned lane = threadIdx.x % 64;
+  float *all = turn[threadIdx.x / 64], *mine = all + lane * (vocab | 1);
+  auto slot = [&](unsigned i) { return i + (__umul24(i, even) >> 16); };    // of element i of the run
   double sum[5] = {0, 0, 0, 0, 0};
-  for (size_t row0 = blockIdx.x * per_block; row0 < a.rows; row0 += gridDim.x * per_block) {
-    const size_t place = row0 + (threadIdx.x >> lanes_log2), row = min(place, a.rows - 1);   // every lane stays, for the permutations
-    const bool live = place < a.rows;
-    const T *in = (const T *)a.logits + (int64_t)row * a.stride;
+  for (size_t row0 = (size_t)blockIdx.x * 256 + threadIdx.x / 64 * 64; row0 < a.rows; row0 += (size_t)gridDim.x * 256) {
+    const unsigned here = (unsigned)min((size_t)64, a.rows - row0), end = here * vocab;
+    const T *in = (const T *)a.logits + (int64_t)row0 * a.stride;
+    asm volatile("" : "+v"(lane));                   // or the compiler holds every element's place across the rows: 256 registers
     T raw[SLOTS];
+    if (a.stride == (int64_t)vocab) {
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) raw[i] = in[min(i * lanes + sub, a.vocab - 1)];
+      for (int k = 0; k < SLOTS; ++k)
+        if (k < SLOTS - 3 || k < (int)vocab) raw[k] = in[min(k * 64 + lane, end - 1)];
+    } else {
+#pragma unroll
+      for (int k = 0; k < SLOTS; ++k) {
+        const unsigned i = min(k * 64 + lane, end - 1), r = __umul24(i, magic) >> 16;
+        if (k < SLOTS - 3 || k < (int)vocab) raw[k] = in[(int64_t)r * a.stride + (i - r * vocab)];
+      }
+    }
+    const size_t row = row0 + min(lane, here - 1);
     const int64_t action = a.actions[row];
     RowInputs q{};
     if (LOSS) q = row_inputs(a, row);
-    const unsigned pick = action >= 0 && action < (int64_t)a.vocab ? (unsigned)action : a.vocab;   // its logit comes out of the registers
-    float x[SLOTS], e[SLOTS], l_a = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < SLOTS; ++k)
+      if (k < SLOTS - 3 || k < (int)vocab) all[slot(k * 64 + lane)] = (float)raw[k];
+    wave_lds_fence();
+    const unsigned pick = action >= 0 && action < (int64_t)vocab ? (unsigned)action : 0;
+    const float l_a = mine[pick];
+    float x[SLOTS], e[SLOTS];
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) x[i] = i < SLOTS - 3 || i < (int)vocab ? mine[i] : -__builtin_inff();
     Softmax w{-__builtin_inff(), 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-      x[i] = i * lanes + sub < a.vocab ? (float)raw[i] : -__builtin_inff();
-      w.m = __builtin_elementwise_maximum(w.m, x[i]);
-      if (i * lanes + sub == pick) l_a = x[i];
-    }
-    l_a = group_max_nan(l_a, lanes);
-    w.m = group_max_nan(w.m, lanes);
+    for (int i = 0; i < SLOTS; i += 2) w.m = max3(w.m, x[i], x[i + 1]);
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
       x[i] = finite_power(x[i], w.m);
@@ -615,28 +636,38 @@ __global__ __launch_bounds__(256) void policy_small_kernel(PolicyArgs a, unsigne
       w.s += e[i];
       w.t = __builtin_fmaf(e[i], x[i], w.t);
     }
-    w.s = group_sum(w.s, lanes);
-    w.t = group_sum(w.t, lanes);
-    const RowTerms o = row_terms(w, action, a.vocab, l_a);
-    if (!live) continue;
-    if (sub == 0) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
-    if (!LOSS) continue;
-    const RowShare share = row_objective(a, q, o);
-    if (sub == 0) {
-      a.dvalues[row] = share.dvalue;
-      for (int i = 0; i < 5; ++i) sum[i] += share.part[i];
-    }
-    const GradTerms k = grad_terms(a, w.m, o, share.g);
-    T *out = (T *)a.dlogits + (int64_t)row * a.dstride;
+    const RowTerms o = row_terms(w, action, vocab, l_a);
+    if (lane < here) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
+    if (LOSS) {
+      const RowShare share = row_objective(a, q, o);
+      if (lane < here) {
+        a.dvalues[row] = share.dvalue;
+        for (int i = 0; i < 5; ++i) sum[i] += share.part[i];
+      }
+      GradTerms k = grad_terms(a, w.m, o, share.g);
+      if (k.nan) k.c0 = __builtin_nanf("");
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-      const unsigned at = i * lanes + sub;
-      float y = e[i] * __builtin_fmaf(x[i], k.c1, k.c0);
-      if (at == pick) y -= k.hit;
-      if (k.nan) y = __builtin_nanf("");
-      if (k.zero) y = 0.f;
-      if (at < a.vocab) out[at] = (T)y;
+      for (int i = 0; i < SLOTS; ++i)
+        if (i < SLOTS - 3 || i < (int)vocab) mine[i] = k.zero ? 0.f : e[i] * __builtin_fmaf(x[i], k.c1, k.c0);
+      if (!k.zero) mine[pick] -= k.hit;              // after a NaN it stays one
+      wave_lds_fence();
+      T *out = (T *)a.dlogits + (int64_t)row0 * a.dstride;
+      asm volatile("" : "+v"(lane));
+      if (a.dstride == (int64_t)vocab) {
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) {
+          const unsigned i = k * 64 + lane;
+          if ((k < SLOTS - 3 || k < (int)vocab) && i < end) out[i] = (T)all[slot(i)];
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) {
+          const unsigned i = k * 64 + lane, r = __umul24(i, magic) >> 16;
+          if ((k < SLOTS - 3 || k < (int)vocab) && i < end) out[(int64_t)r * a.dstride + (i - r * vocab)] = (T)all[slot(i)];
+        }
+      }
     }
+    wave_lds_fence();
   }
   if (LOSS) put_block(a, sum, red);
 }
@@ -973,7 +1004,7 @@ enum Route { kSmall, kGroup, kRow, kSplit };
 
 struct Plan {
   Route route = kRow;
-  unsigned lanes_log2 = 0, chunks = 0;             // kSmall, kGroup: lanes of a row; kSplit: chunks of a row
+  unsigned lanes_log2 = 0, chunks = 0;             // kGroup: lanes of a row; kSplit: chunks of a row
   unsigned blocks = 0;                             // kSmall, kGroup: workgroups, which walk over the rows
   size_t records = 0;                              // of the objective
   size_t o_slices = 0, o_ticket = 0, o_parts = 0, o_picked = 0, bytes = 0;
@@ -990,7 +1021,8 @@ Plan plan_of(size_t rows, size_t vocab, bool loss) {
   Plan p;
   if (vocab <= kGroupVocab) {
     p.route = vocab <= kSmallVocab ? kSmall : kGroup;
-    while ((p.route == kSmall ? 8u : 32u) << p.lanes_log2 < vocab) ++p.lanes_log2;
+    if (p.route == kGroup)
+      while (32u << p.lanes_log2 < vocab) ++p.lanes_log2;
     const size_t per = 256u >> p.lanes_log2;
     p.blocks = (unsigned)std::min<size_t>((rows + per - 1) / per, kGroupBlocks);
   } else if (rows < kSplitRows && vocab > (loss ? kSplitLoss : kSplitStats)) {
@@ -1019,13 +1051,17 @@ void launch_group(const Plan &p, const PolicyArgs &a, hipStream_t s) {
     else hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 4>), grid, block, 0, s, a, p.lanes_log2);
     return;
   }
-  const unsigned slots = (a.vocab + (1u << p.lanes_log2) - 1) >> p.lanes_log2;
-  if (slots <= 2) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 2>), grid, block, 0, s, a, p.lanes_log2);
-  else if (slots <= 4) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 4>), grid, block, 0, s, a, p.lanes_log2);
-  else if (slots == 5) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 5>), grid, block, 0, s, a, p.lanes_log2);
-  else if (slots == 6) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 6>), grid, block, 0, s, a, p.lanes_log2);
-  else if (slots == 7) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 7>), grid, block, 0, s, a, p.lanes_log2);
-  else hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 8>), grid, block, 0, s, a, p.lanes_log2);
+  const unsigned magic = (65536 + a.vocab - 1) / a.vocab;       // exact for the 64 * vocab elements of a wave's rows
+  switch ((a.vocab + 3) / 4) {
+    case 1: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 4>), grid, block, 0, s, a, magic); break;
+    case 2: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 8>), grid, block, 0, s, a, magic); break;
+    case 3: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 12>), grid, block, 0, s, a, magic); break;
+    case 4: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 16>), grid, block, 0, s, a, magic); break;
+    case 5: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 20>), grid, block, 0, s, a, magic); break;
+    case 6: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 24>), grid, block, 0, s, a, magic); break;
+    case 7: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 28>), grid, block, 0, s, a, magic); break;
+    default: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 32>), grid, block, 0, s, a, magic);
+  }
 }
 
 template <typename T>
