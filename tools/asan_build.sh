@@ -6,9 +6,9 @@ set -e
 cd "$(dirname "$0")/.."
 mkdir -p build_asan && cd build_asan
 H=/opt/rocm/bin/hipcc
-F="--offload-arch=gfx950 -O1 -g -std=c++17 -fPIC -ffp-contract=off -Xarch_host -fsanitize=address -Xarch_host -fno-omit-frame-pointer"
-for f in ppo_xp device_shuffle rnorm; do $H $F -c -o $f.o ../ppo_amd/csrc/$f.hip -I../ppo_amd/csrc; done
-$H --offload-arch=gfx950 -shared -fsanitize=address -fno-gpu-sanitize -o libppo_xp.so ppo_xp.o device_shuffle.o rnorm.o -ldl
+F="--offload-arch=gfx950 -O1 -g -std=c++17 -fPIC -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops -Xarch_host -fsanitize=address -Xarch_host -fno-omit-frame-pointer"
+for f in ppo_xp device_shuffle rnorm policy qrows; do $H $F -c -o $f.o ../ppo_amd/csrc/$f.hip -I../ppo_amd/csrc; done
+$H --offload-arch=gfx950 -shared -fsanitize=address -fno-gpu-sanitize -o libppo_xp.so ppo_xp.o device_shuffle.o rnorm.o policy.o qrows.o -ldl
 rm -f *.o
 C=/opt/rocm/lib/llvm/bin/clang++
 for t in abi_stress test_reference_cases; do
