@@ -112,7 +112,8 @@ class ExperienceBuffer:
     def new_quantized(cls, num_envs, row_size, capacity, format="int8", group=64, dtype=None, gamma=0.99, lam=0.95, device=0):
         """A buffer whose observation rows (hidden states of `row_size` elements, f32 / bf16 / f16) are kept in 8 or 4 bits: quantised as
         add_experience* writes them, read back as `dtype` (default f32) by the minibatches of a pass (quant.QuantizedRows).  The
-        other streams and the pass itself are the ordinary ones; rows are written and read on torch's current stream."""
+        other streams and the pass itself are the ordinary ones; rows are written and read on torch's current stream, a minibatch's
+        when the iterator yields it: insert again only after that (as with streaming passes)."""
         import torch
         from .quant import QuantizedRows
         self = cls(num_envs, 1, capacity, gamma, lam, device)      # the handle's own rows: one unused float

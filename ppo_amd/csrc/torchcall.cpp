@@ -98,6 +98,11 @@ at::Tensor result(PyObject *o, const at::Tensor &like, const char *what, Matrix 
   return out;
 }
 
+// A caller's `out` changes under autograd's eyes: what was saved of it for a backward pass is known to be stale.
+void written(PyObject *o, const at::Tensor &out) {
+  if (o != Py_None && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
+
 void *stream_of(int device) {
   PyObject *d = PyLong_FromLong(device), *r = d ? PyObject_CallOneArg(g_stream, d) : nullptr;
   Py_XDECREF(d);
@@ -193,6 +198,7 @@ PyObject *shape(PyObject *const *a) {                       // logits, rules, ou
   const ppo_xp_logit_rules r = rules_of(l, a + 1);
   Matrix o;
   at::Tensor out = result(a[1 + RULES], t, "shape_logits", o);
+  written(a[1 + RULES], out);
   done(launch(g_shape, l.device, stream_of(l.device), l.dtype, l.p, l.stride, o.p, o.stride, l.rows, l.cols, &r));
   return THPVariable_Wrap(out);
 }
@@ -207,6 +213,7 @@ PyObject *shape_backward(PyObject *const *a) {              // grad, logits, rul
   const ppo_xp_logit_rules r = rules_of(l, a + 2);
   Matrix o;
   at::Tensor out = result(a[2 + RULES], g, who, o);
+  written(a[2 + RULES], out);
   done(launch(g_shape_backward, l.device, stream_of(l.device), l.dtype, m.p, m.stride, l.p, l.stride, o.p, o.stride, l.rows, l.cols, &r));
   return THPVariable_Wrap(out);
 }
@@ -230,6 +237,7 @@ PyObject *stats(PyObject *const *a) {                       // logits, actions
   const int64_t ws = (int64_t)(g_workspace(l.rows, l.cols, 0) + 15) / 16 * 4;
   at::Tensor buf = at::empty({ws + 2 * l.rows}, floats(t));
   float *p = buf.data_ptr<float>();
+  if (l.cols == 0) buf.zero_();
   done(launch(g_stats, l.device, stream_of(l.device), l.dtype, l.p, l.stride, (const int64_t *)actions, p + ws, p + ws + l.rows, l.rows, l.cols, p, ws * 4));
   PyObject *r = PyTuple_New(2);
   if (!r) throw Raised{};
@@ -269,6 +277,7 @@ PyObject *loss(PyObject *const *a) {                        // logits, values, b
   at::Tensor buf = at::empty({ws + 3 * n + 6}, floats(t));
   float *p = buf.data_ptr<float>(), *q = p + ws;
   if (l.rows == 0 || l.cols == 0) buf.zero_();
+  written(a[7], out);
   done(launch(g_loss, l.device, stream_of(l.device), l.dtype, l.p, l.stride, &b, clip, ent, vf, denom, o.p, o.stride, q, q + n, q + 2 * n, q + 3 * n, l.rows,
               l.cols, p, ws * 4));
   PyObject *r = PyTuple_New(5);

@@ -579,3 +579,56 @@ def test_refusals_on_the_gpu():
     b.returns = v[:3]
     with pytest.raises(PpoXpPanic):
         ppo_amd.policy_loss(x, v, b)
+
+
+# ---- what a caller's tensors are left as ----------------------------------------------------------------------------------
+
+def test_written_in_place_is_seen_by_autograd():
+    import ppo_amd
+    g = gen(21)
+    R, V = 4, 40
+    x = randn(g, R, V).requires_grad_()
+    z = torch.zeros(R, device="cuda")
+    batch = batch_of(g, x.detach(), torch.zeros(R, dtype=torch.int64, device="cuda"))
+    for write in (lambda y: ppo_amd.shape_logits(y, temperature=0.5, out=y),
+                  lambda y: ppo_amd.shape_logits_backward(torch.ones_like(y), x.detach(), temperature=0.5, out=y),
+                  lambda y: ppo_amd.policy_loss(y, z, batch, out=y)):
+        y = x.exp()                                        # saves its output for the backward pass
+        write(y)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        y = x.exp()                                        # ... and one that is only read stays good
+        ppo_amd.shape_logits(y, temperature=0.5)
+        ppo_amd.policy_loss(y, z, batch)
+        y.sum().backward()
+    with torch.inference_mode():
+        y = x.exp()
+        want = ppo_amd.shape_logits(y, temperature=0.5)
+        assert torch.equal(ppo_amd.shape_logits(y, temperature=0.5, out=y), want)
+
+
+def test_no_tokens_and_no_rows():
+    import ppo_amd
+    for R, V in ((0, 5), (3, 0), (0, 0)):
+        x = torch.zeros(R, V, device="cuda")
+        nlp, ent = ppo_amd.action_stats(x, torch.zeros(R, dtype=torch.int64, device="cuda"))
+        assert nlp.shape == ent.shape == (R,) and torch.all(nlp == 0) and torch.all(ent == 0)
+        assert ppo_amd.shape_logits(x).shape == (R, V)
+
+
+def test_results_are_ordinary_tensors():
+    """They share memory with a workspace but not with each other: copies, views, pickles and in-place changes are theirs alone."""
+    import copy
+    import ppo_amd
+    g, x, a = policy_inputs(64, 50, F32, 5)
+    z = torch.zeros(64, device="cuda")
+    r = ppo_amd.policy_loss(x, z, batch_of(g, x, a))
+    nlp, ent = ppo_amd.action_stats(x, a)
+    parts = [r.stats, r.dvalues, r.neglogps, r.entropies, nlp, ent]
+    before = [p.clone() for p in parts]
+    for k, p in enumerate(parts):
+        assert p.is_contiguous() and not p.requires_grad and p._base is None
+        assert torch.equal(copy.deepcopy(p), before[k]) and torch.equal(p.reshape(-1, 1)[:, 0], before[k])
+        p.add_(1.0)
+        assert all(torch.equal(q, before[j]) for j, q in enumerate(parts) if j > k)
+        assert torch.equal(p, before[k] + 1.0)
