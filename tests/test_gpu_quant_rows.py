@@ -230,3 +230,22 @@ def test_refusals():
             call()
     with pytest.raises(PpoXpPanic):
         ppo_amd.QuantizedRows(0, 64).read(i)
+
+
+def test_refuses_tensors_that_no_longer_fit():
+    """codes and scales are attributes: exchanged ones are looked at before they are used."""
+    import ppo_amd
+    from ppo_amd import PpoXpPanic
+    x = torch.zeros(8, 64, device="cuda")
+    good = ppo_amd.QuantizedRows(8, 64, "int8", 32)
+    for codes, scales in ((good.codes[:4], good.scales), (good.codes, good.scales[:4]), (good.codes[:, :63], good.scales), (good.codes, good.scales[:, :1]),
+                          (good.codes.cpu(), good.scales), (good.codes, good.scales.cpu()), (good.codes.int(), good.scales), (good.codes, good.scales.double()),
+                          (good.codes.t().contiguous().t(), good.scales), (good.codes[0], good.scales)):
+        s = ppo_amd.QuantizedRows.of(good.codes, good.scales, 64, "int8", 32)
+        s.codes, s.scales = codes, scales
+        for call in (lambda: s.write(x), lambda: s.read()):
+            with pytest.raises(PpoXpPanic):
+                call()
+    s = ppo_amd.QuantizedRows(8, 64, "int8", 32)
+    s.codes, s.scales = torch.ones_like(good.codes), torch.full_like(good.scales, 2.0)      # others of the same shapes are the store now
+    assert torch.all(s.read() == 2.0)

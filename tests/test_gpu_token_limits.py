@@ -161,3 +161,48 @@ def test_current_device_and_autograd_state_are_left_alone():
     d = ppo_amd.shape_logits_backward(torch.ones(3, 50, device="cuda"), x, temperature=2.0)
     x.backward(d)
     assert torch.all(x.grad == 0.5)
+
+
+def test_threads_call_at_once():
+    """Calls release the interpreter while they launch: each thread on a stream of its own gets what it gets alone."""
+    import threading
+    import ppo_amd
+    shapes = [(300, 18, F32), (64, 700, BF16), (4, 70001, F16), (3, 150000, F32)]
+    jobs, wrong = [], []
+    for k, (R, V, dtype) in enumerate(shapes):
+        g, x, a = policy_inputs(R, V, dtype, 100 + k)
+        b = batch_of(g, x, a)
+        hist = torch.randint(0, V, (R, 33), generator=g, device="cuda")
+        store = ppo_amd.QuantizedRows(R, 70, "int8", 32)
+        rows = randn(g, R, 70)
+
+        def work(x=x, a=a, b=b, hist=hist, store=store, rows=rows):
+            y = ppo_amd.shape_logits(x, history=hist, repetition=1.3, frequency=0.1)
+            store.write(rows)
+            r = ppo_amd.policy_loss(y, b.new_values, b)
+            d = ppo_amd.shape_logits_backward(r.dlogits, x, history=hist, repetition=1.3)
+            return [y, *ppo_amd.action_stats(y, a), r.stats, r.dvalues, d, store.read()]
+        jobs.append((work, work()))
+    torch.cuda.synchronize()
+
+    def run(work, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got = [work() for _ in range(30)]
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(p, q) for out in got for p, q in zip(out, want)):
+                    wrong.append("results differ")
+                try:
+                    ppo_amd.shape_logits(want[0], repetition=-1.0)
+                    wrong.append("not refused")
+                except ppo_amd.PpoXpPanic as e:
+                    if "repetition" not in str(e):
+                        wrong.append(str(e))
+        except Exception as e:  # noqa: BLE001
+            wrong.append(repr(e))
+    threads = [threading.Thread(target=run, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
