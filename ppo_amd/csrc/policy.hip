@@ -436,8 +436,9 @@ __device__ __forceinline__ void load_row(Raw8<T> *r, const T *in, unsigned lane,
 }
 
 // NV vectors in registers, `step` elements apart from element e0 on.  Returns whether the whole wave went the short way, which
-// its gradient may then go as well.
-template <int NV, typename T>
+// its gradient may then go as well.  KEEP: few enough vectors to hold their floats from the maximum to the sums, one conversion an
+// element less (statistics of 4096 x 32768 bf16 49.0 us against 51.0).
+template <int NV, bool KEEP = false, typename T>
 __device__ __forceinline__ bool row_softmax(Softmax &w, const Raw8<T> *r, const T *in, unsigned e0, unsigned step, Span at) {
   float least = 0.f;
 #pragma unroll
@@ -455,7 +456,7 @@ __device__ __forceinline__ bool row_softmax(Softmax &w, const Raw8<T> *r, const 
     for (int k = 0; k < NV; ++k) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float x = __builtin_fmaf(r[k].fresh(i), kLog2e, -p.m2), e = exp2_fast(x);
+        const float x = __builtin_fmaf(KEEP ? r[k].get(i) : r[k].fresh(i), kLog2e, -p.m2), e = exp2_fast(x);
         w.s += e;
         w.t = __builtin_fmaf(e, x, w.t);
       }
@@ -728,7 +729,7 @@ __global__ __launch_bounds__(THREADS) void policy_stats_row_kernel(PolicyArgs a)
       const Span part{e0 ? 0u : at.first, min(at.end - e0, kStatsVecs * THREADS * 8u)};
       load_row<kStatsVecs>(r, in + e0, threadIdx.x, THREADS, part);
       Softmax q{-__builtin_inff(), 0.f, 0.f};
-      row_softmax<kStatsVecs>(q, r, in + e0, threadIdx.x * 8, THREADS * 8, part);
+      row_softmax<kStatsVecs, true>(q, r, in + e0, threadIdx.x * 8, THREADS * 8, part);
       const float m = __builtin_elementwise_maximum(w.m, q.m);
       rebase(w.m, m, w.s, w.t);
       rebase(q.m, m, q.s, q.t);
@@ -812,7 +813,7 @@ __global__ __launch_bounds__(256) void policy_split_kernel(PolicyArgs a, unsigne
   Softmax w{-__builtin_inff(), 0.f, 0.f};
   const unsigned len = min(a.vocab - c0, kSplitChunk);
   load_row<kSplitVecs>(r, in + c0, threadIdx.x, 256, Span{0, len});
-  row_softmax<kSplitVecs>(w, r, in + c0, threadIdx.x * 8, 2048, Span{0, len});
+  row_softmax<kSplitVecs, true>(w, r, in + c0, threadIdx.x * 8, 2048, Span{0, len});
   w = block_softmax(w, red);
   if (threadIdx.x == 0) {
     parts[blockIdx.x] = w;
