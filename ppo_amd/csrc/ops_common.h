@@ -150,10 +150,23 @@ __device__ __forceinline__ unsigned group_max_bits(unsigned x, unsigned lanes) {
     return __builtin_bit_cast(float, max(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)));
   }));
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double x) {
+  const u32x2 v = __builtin_bit_cast(u32x2, x);
+  const u32x2 o = {(unsigned)__builtin_amdgcn_update_dpp(0, (int)v.x, CTRL, ROWS, 0xf, false),
+                   (unsigned)__builtin_amdgcn_update_dpp(0, (int)v.y, CTRL, ROWS, 0xf, false)};
+  return x + __builtin_bit_cast(double, o);
+}
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-  return x;
+  x = dpp_add<0x128, 0xf>(x);
+  x = dpp_add<0x124, 0xf>(x);
+  x = dpp_add<0x122, 0xf>(x);
+  x = dpp_add<0x121, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);
+  x = dpp_add<0x143, 0xc>(x);
+  const u32x2 v = __builtin_bit_cast(u32x2, x);
+  const u32x2 last = {(unsigned)__builtin_amdgcn_readlane((int)v.x, 63), (unsigned)__builtin_amdgcn_readlane((int)v.y, 63)};
+  return __builtin_bit_cast(double, last);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------

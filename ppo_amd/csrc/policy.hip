@@ -923,10 +923,11 @@ __global__ __launch_bounds__(960) void policy_stats_kernel(const double *partial
     __threadfence();
     sum_records(slices, kStatsBlocks, 0, gridDim.x, s, red);
   }
-  if (threadIdx.x) return;
-  for (int k = 0; k < 5; ++k) s[k] /= denom;
-  stats[0] = (float)(s[0] + (double)vf * s[1] - (double)ent * s[2]);
-  for (int k = 0; k < 5; ++k) stats[1 + k] = (float)s[k];
+  if (threadIdx.x >= 6) return;                      // a division each, side by side
+  double x = s[0] + (double)vf * s[1] - (double)ent * s[2];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) x = threadIdx.x == 1 + k ? s[k] : x;
+  stats[threadIdx.x] = (float)(x / denom);
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
