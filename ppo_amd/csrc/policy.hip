@@ -600,12 +600,14 @@ __device__ __forceinline__ void put_block(const PolicyArgs &a, const double sum[
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
 }
 
-// Up to kSmallVocab tokens, the action sets of ordinary environments: a lane a row, since what a row costs beside its elements is as
-// much as 15 of them.  A wave's 64 rows come in and leave as one run of elements, 64 neighbours an access, and are turned in shared
-// memory, where rows lie an odd number of floats apart, free of bank conflicts.  SLOTS elements a lane, a multiple of 4, the last 3
-// perhaps beyond the row.  Memory bounds it: the objective of 1048576 x 32 f32 moves 306 MB in 60 us; with several lanes a row and no
-// turning it took 120 us, 262144 x 18 f32 18.9 us against 16.2 us, statistics of 262144 x 32 f32 7.9 against 9.2 us.
-constexpr unsigned kSmallVocab = 32, kGroupBlocks = 1536;
+// Up to 64 tokens (statistics: 56), the action sets of ordinary environments: a lane a row, since what a row costs beside its elements
+// is as much as 15 of them.  A wave's 64 rows come in and leave as one run of elements, 64 neighbours an access, and are turned in
+// shared memory, where rows lie an odd number of floats apart, free of bank conflicts.  SLOTS elements a lane, the last of them perhaps
+// beyond the row.  Memory bounds it: the objective of 1048576 x 32 f32 moves 306 MB in 59 us, of 262144 x 18 f32 49 MB in 15 us.  Rows
+// over several lanes, as policy_group_kernel has them, against it, us: objective f32 838860 x 40 101 | 58, 532610 x 63 118 | 69,
+// 524288 x 64 75 | 66, bf16 599186 x 56 92 | 58, 524288 x 64 62 | 66; statistics f32 599186 x 56 44 | 31, 524288 x 64 31 | 29, bf16 24 | 25
+// and 17 | 30 (two waves a SIMD are all that fit beside the turned rows).
+constexpr unsigned kSmallVocab = 64, kSmallStats = 56, kGroupBlocks = 1536;
 
 __device__ __forceinline__ void wave_lds_fence() {            // what the wave's lanes wrote to LDS, its other lanes read afterwards
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -614,13 +616,14 @@ __device__ __forceinline__ void wave_lds_fence() {            // what the wave's
 }
 
 template <typename T, bool LOSS, int SLOTS>
-__global__ __launch_bounds__(256, 4) void policy_small_kernel(PolicyArgs a, unsigned magic) {   // magic: 2^16 / vocab, rounded up
+__global__ __launch_bounds__(256, SLOTS <= 32 ? 4 : 2) void policy_small_kernel(PolicyArgs a, unsigned magic) {   // magic: 2^20 / vocab, rounded up
+  constexpr int LEAST = SLOTS <= 32 ? SLOTS - 3 : SLOTS - 7;   // tokens of a row at least
   __shared__ double red[4][5];
   __shared__ float turn[4][64 * (SLOTS + 1)];
   const unsigned vocab = a.vocab, even = vocab % 2 ? 0 : magic;
   unsigned lane = threadIdx.x % 64;
   float *all = turn[threadIdx.x / 64], *mine = all + lane * (vocab | 1);
-  auto slot = [&](unsigned i) { return i + (__umul24(i, even) >> 16); };    // of element i of the run
+  auto slot = [&](unsigned i) { return i + (__umul24(i, even) >> 20); };    // of element i of the run
   double sum[5] = {0, 0, 0, 0, 0};
   for (size_t row0 = (size_t)blockIdx.x * 256 + threadIdx.x / 64 * 64; row0 < a.rows; row0 += (size_t)gridDim.x * 256) {
     const unsigned here = (unsigned)min((size_t)64, a.rows - row0), end = here * vocab;
@@ -630,12 +633,12 @@ __global__ __launch_bounds__(256, 4) void policy_small_kernel(PolicyArgs a, unsi
     if (a.stride == (int64_t)vocab) {
 #pragma unroll
       for (int k = 0; k < SLOTS; ++k)
-        if (k < SLOTS - 3 || k < (int)vocab) raw[k] = in[min(k * 64 + lane, end - 1)];
+        if (k < LEAST || k < (int)vocab) raw[k] = in[min(k * 64 + lane, end - 1)];
     } else {
 #pragma unroll
       for (int k = 0; k < SLOTS; ++k) {
-        const unsigned i = min(k * 64 + lane, end - 1), r = __umul24(i, magic) >> 16;
-        if (k < SLOTS - 3 || k < (int)vocab) raw[k] = in[(int64_t)r * a.stride + (i - r * vocab)];
+        const unsigned i = min(k * 64 + lane, end - 1), r = __umul24(i, magic) >> 20;
+        if (k < LEAST || k < (int)vocab) raw[k] = in[(int64_t)r * a.stride + (i - r * vocab)];
       }
     }
     const size_t row = row0 + min(lane, here - 1);
@@ -644,13 +647,13 @@ __global__ __launch_bounds__(256, 4) void policy_small_kernel(PolicyArgs a, unsi
     if (LOSS) q = row_inputs(a, row);
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k)
-      if (k < SLOTS - 3 || k < (int)vocab) all[slot(k * 64 + lane)] = (float)raw[k];
+      if (k < LEAST || k < (int)vocab) all[slot(k * 64 + lane)] = (float)raw[k];
     wave_lds_fence();
     const unsigned pick = action >= 0 && action < (int64_t)vocab ? (unsigned)action : 0;
     const float l_a = mine[pick];
     float x[SLOTS], e[SLOTS];
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) x[i] = i < SLOTS - 3 || i < (int)vocab ? mine[i] : -__builtin_inff();
+    for (int i = 0; i < SLOTS; ++i) x[i] = i < LEAST || i < (int)vocab ? mine[i] : -__builtin_inff();
     Softmax w{-__builtin_inff(), 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < SLOTS; i += 2) w.m = max3(w.m, x[i], x[i + 1]);
@@ -673,7 +676,7 @@ __global__ __launch_bounds__(256, 4) void policy_small_kernel(PolicyArgs a, unsi
       if (k.nan) k.c0 = __builtin_nanf("");
 #pragma unroll
       for (int i = 0; i < SLOTS; ++i)
-        if (i < SLOTS - 3 || i < (int)vocab) mine[i] = k.zero ? 0.f : e[i] * __builtin_fmaf(x[i], k.c1, k.c0);
+        if (i < LEAST || i < (int)vocab) mine[i] = k.zero ? 0.f : e[i] * __builtin_fmaf(x[i], k.c1, k.c0);
       if (!k.zero) mine[pick] -= k.hit;              // after a NaN it stays one
       wave_lds_fence();
       T *out = (T *)a.dlogits + (int64_t)row0 * a.dstride;
@@ -682,13 +685,13 @@ __global__ __launch_bounds__(256, 4) void policy_small_kernel(PolicyArgs a, unsi
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k) {
           const unsigned i = k * 64 + lane;
-          if ((k < SLOTS - 3 || k < (int)vocab) && i < end) out[i] = (T)all[slot(i)];
+          if ((k < LEAST || k < (int)vocab) && i < end) out[i] = (T)all[slot(i)];
         }
       } else {
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k) {
-          const unsigned i = k * 64 + lane, r = __umul24(i, magic) >> 16;
-          if ((k < SLOTS - 3 || k < (int)vocab) && i < end) out[(int64_t)r * a.dstride + (i - r * vocab)] = (T)all[slot(i)];
+          const unsigned i = k * 64 + lane, r = __umul24(i, magic) >> 20;
+          if ((k < LEAST || k < (int)vocab) && i < end) out[(int64_t)r * a.dstride + (i - r * vocab)] = (T)all[slot(i)];
         }
       }
     }
@@ -1046,7 +1049,7 @@ constexpr size_t kSplitRows = 128, kSplitLoss = 65536, kSplitStats = 98304;   //
 Plan plan_of(size_t rows, size_t vocab, bool loss) {
   Plan p;
   if (vocab <= kGroupVocab) {
-    p.route = vocab <= kSmallVocab ? kSmall : kGroup;
+    p.route = vocab <= (loss ? kSmallVocab : kSmallStats) ? kSmall : kGroup;
     if (p.route == kGroup)
       while (32u << p.lanes_log2 < vocab) ++p.lanes_log2;
     const size_t per = 256u >> p.lanes_log2;
@@ -1077,8 +1080,8 @@ void launch_group(const Plan &p, const PolicyArgs &a, hipStream_t s) {
     else hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 4>), grid, block, 0, s, a, p.lanes_log2);
     return;
   }
-  const unsigned magic = (65536 + a.vocab - 1) / a.vocab;       // exact for the 64 * vocab elements of a wave's rows
-  switch ((a.vocab + 3) / 4) {
+  const unsigned magic = ((1u << 20) + a.vocab - 1) / a.vocab;       // exact for the 64 * vocab elements of a wave's rows
+  switch (a.vocab <= 32 ? (a.vocab + 3) / 4 : (a.vocab + 7) / 8 * 2) {
     case 1: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 4>), grid, block, 0, s, a, magic); break;
     case 2: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 8>), grid, block, 0, s, a, magic); break;
     case 3: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 12>), grid, block, 0, s, a, magic); break;
@@ -1086,7 +1089,12 @@ void launch_group(const Plan &p, const PolicyArgs &a, hipStream_t s) {
     case 5: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 20>), grid, block, 0, s, a, magic); break;
     case 6: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 24>), grid, block, 0, s, a, magic); break;
     case 7: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 28>), grid, block, 0, s, a, magic); break;
-    default: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 32>), grid, block, 0, s, a, magic);
+    case 8: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 32>), grid, block, 0, s, a, magic); break;
+    case 10: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 40>), grid, block, 0, s, a, magic); break;
+    case 12: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 48>), grid, block, 0, s, a, magic); break;
+    case 14: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 56>), grid, block, 0, s, a, magic); break;
+    default:
+      if constexpr (LOSS) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 64>), grid, block, 0, s, a, magic);
   }
 }
 
