@@ -600,14 +600,12 @@ __device__ __forceinline__ void put_block(const PolicyArgs &a, const double sum[
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.ticket = 0;
 }
 
-// Up to 64 tokens (statistics: 56), the action sets of ordinary environments: a lane a row, since what a row costs beside its elements
-// is as much as 15 of them.  A wave's 64 rows come in and leave as one run of elements, 64 neighbours an access, and are turned in
-// shared memory, where rows lie an odd number of floats apart, free of bank conflicts.  SLOTS elements a lane, the last of them perhaps
-// beyond the row.  Memory bounds it: the objective of 1048576 x 32 f32 moves 306 MB in 59 us, of 262144 x 18 f32 49 MB in 15 us.  Rows
-// over several lanes, as policy_group_kernel has them, against it, us: objective f32 838860 x 40 101 | 58, 532610 x 63 118 | 69,
-// 524288 x 64 75 | 66, bf16 599186 x 56 92 | 58, 524288 x 64 62 | 66; statistics f32 599186 x 56 44 | 31, 524288 x 64 31 | 29, bf16 24 | 25
-// and 17 | 30 (two waves a SIMD are all that fit beside the turned rows).
-constexpr unsigned kSmallVocab = 64, kSmallStats = 56, kGroupBlocks = 1536;
+// Action sets of ordinary environments, and rows of some hundred tokens that do not fill the lanes of policy_group_kernel: a wave's rows
+// come in and leave as one run of elements, 64 neighbours an access, and are turned in shared memory, where they lie an odd number of
+// floats apart, free of bank conflicts.  Up to 48 tokens a lane has a row, since what a row costs beside its elements is as much as 15 of
+// them; longer ones are SPREAD over 2, 4, ... lanes, element i with lane i of them.  SLOTS elements a lane, the last of them perhaps
+// beyond the row.  Memory bounds it (objective of 1048576 x 32 f32: 306 MB in 59 us, of 262144 x 18 f32: 49 MB in 15 us).
+constexpr unsigned kGroupBlocks = 1536;
 
 __device__ __forceinline__ void wave_lds_fence() {            // what the wave's lanes wrote to LDS, its other lanes read afterwards
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -615,48 +613,55 @@ __device__ __forceinline__ void wave_lds_fence() {            // what the wave's
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <typename T, bool LOSS, int SLOTS>
-__global__ __launch_bounds__(256, SLOTS <= 32 ? 4 : 2) void policy_small_kernel(PolicyArgs a, unsigned magic) {   // magic: 2^20 / vocab, rounded up
-  constexpr int LEAST = SLOTS <= 32 ? SLOTS - 3 : SLOTS - 7;   // tokens of a row at least
+template <typename T, bool LOSS, int SLOTS, bool SPREAD>
+__global__ __launch_bounds__(256, SLOTS <= 32 ? 4 : 2) void policy_small_kernel(PolicyArgs a, unsigned magic, unsigned lanes_log2) {   // magic: 2^22 / vocab, rounded up
+  constexpr int LEAST = SLOTS <= 32 && !SPREAD ? SLOTS - 3 : SLOTS - 7, FULL = SPREAD ? LEAST - 1 : LEAST;   // slots in use at least, and up to their end
   __shared__ double red[4][5];
   __shared__ float turn[4][64 * (SLOTS + 1)];
   const unsigned vocab = a.vocab, even = vocab % 2 ? 0 : magic;
+  const unsigned lg = SPREAD ? lanes_log2 : 0, lanes = 1u << lg, wave_rows = 64u >> lg;
+  const int slots = (int)((vocab + lanes - 1) >> lg);
   unsigned lane = threadIdx.x % 64;
-  float *all = turn[threadIdx.x / 64], *mine = all + lane * (vocab | 1);
-  auto slot = [&](unsigned i) { return i + (__umul24(i, even) >> 20); };    // of element i of the run
+  float *all = turn[threadIdx.x / 64];
+  auto place = [&]() { return all + (lane >> lg) * (vocab | 1) + (lane & (lanes - 1)); };   // of the lane's first element
+  auto slot = [&](unsigned i) { return i + (__umul24(i, even) >> 22); };    // of element i of the run
   double sum[5] = {0, 0, 0, 0, 0};
-  for (size_t row0 = (size_t)blockIdx.x * 256 + threadIdx.x / 64 * 64; row0 < a.rows; row0 += (size_t)gridDim.x * 256) {
-    const unsigned here = (unsigned)min((size_t)64, a.rows - row0), end = here * vocab;
+  for (size_t row0 = ((size_t)blockIdx.x * 4 + threadIdx.x / 64) * wave_rows; row0 < a.rows; row0 += (size_t)gridDim.x * 4 * wave_rows) {
+    const unsigned here = (unsigned)min((size_t)wave_rows, a.rows - row0), end = here * vocab;
     const T *in = (const T *)a.logits + (int64_t)row0 * a.stride;
     asm volatile("" : "+v"(lane));                   // or the compiler holds every element's place across the rows: 256 registers
     T raw[SLOTS];
     if (a.stride == (int64_t)vocab) {
 #pragma unroll
       for (int k = 0; k < SLOTS; ++k)
-        if (k < LEAST || k < (int)vocab) raw[k] = in[min(k * 64 + lane, end - 1)];
+        if (k < LEAST || k < slots) raw[k] = in[min(k * 64 + lane, end - 1)];
     } else {
 #pragma unroll
       for (int k = 0; k < SLOTS; ++k) {
-        const unsigned i = min(k * 64 + lane, end - 1), r = __umul24(i, magic) >> 20;
-        if (k < LEAST || k < (int)vocab) raw[k] = in[(int64_t)r * a.stride + (i - r * vocab)];
+        const unsigned i = min(k * 64 + lane, end - 1), r = __umul24(i, magic) >> 22;
+        if (k < LEAST || k < slots) raw[k] = in[(int64_t)r * a.stride + (i - r * vocab)];
       }
     }
-    const size_t row = row0 + min(lane, here - 1);
+    const unsigned own = lane >> lg, sub = lane & (lanes - 1);
+    const size_t row = row0 + min(own, here - 1);
+    const bool puts = own < here && sub == 0;
     const int64_t action = a.actions[row];
     RowInputs q{};
     if (LOSS) q = row_inputs(a, row);
 #pragma unroll
     for (int k = 0; k < SLOTS; ++k)
-      if (k < LEAST || k < (int)vocab) all[slot(k * 64 + lane)] = (float)raw[k];
+      if (k < LEAST || k < slots) all[slot(k * 64 + lane)] = (float)raw[k];
     wave_lds_fence();
     const unsigned pick = action >= 0 && action < (int64_t)vocab ? (unsigned)action : 0;
-    const float l_a = mine[pick];
+    float *mine = place();
+    const float l_a = mine[(int)pick - (int)sub];
     float x[SLOTS], e[SLOTS];
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) x[i] = i < LEAST || i < (int)vocab ? mine[i] : -__builtin_inff();
+    for (int i = 0; i < SLOTS; ++i) x[i] = i < FULL || (i << lg) + sub < vocab ? mine[i << lg] : -__builtin_inff();
     Softmax w{-__builtin_inff(), 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < SLOTS; i += 2) w.m = max3(w.m, x[i], x[i + 1]);
+    if (SPREAD) w.m = group_max_nan(w.m, lanes);
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
       x[i] = finite_power(x[i], w.m);
@@ -664,20 +669,26 @@ __global__ __launch_bounds__(256, SLOTS <= 32 ? 4 : 2) void policy_small_kernel(
       w.s += e[i];
       w.t = __builtin_fmaf(e[i], x[i], w.t);
     }
+    if (SPREAD) {
+      w.s = group_sum(w.s, lanes);
+      w.t = group_sum(w.t, lanes);
+    }
     const RowTerms o = row_terms(w, action, vocab, l_a);
-    if (lane < here) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
+    if (puts) { a.neglogps[row] = o.nlp; a.entropies[row] = o.ent; }
     if (LOSS) {
       const RowShare share = row_objective(a, q, o);
-      if (lane < here) {
+      if (puts) {
         a.dvalues[row] = share.dvalue;
         for (int i = 0; i < 5; ++i) sum[i] += share.part[i];
       }
       GradTerms k = grad_terms(a, w.m, o, share.g);
       if (k.nan) k.c0 = __builtin_nanf("");
+      if (SPREAD) asm volatile("" : "+v"(lane));
+      mine = place();
 #pragma unroll
       for (int i = 0; i < SLOTS; ++i)
-        if (i < LEAST || i < (int)vocab) mine[i] = k.zero ? 0.f : e[i] * __builtin_fmaf(x[i], k.c1, k.c0);
-      if (!k.zero) mine[pick] -= k.hit;              // after a NaN it stays one
+        if (i < FULL || (i << lg) + sub < vocab) mine[i << lg] = k.zero ? 0.f : e[i] * __builtin_fmaf(x[i], k.c1, k.c0);
+      if (!k.zero && (pick & (lanes - 1)) == sub) mine[pick - sub] -= k.hit;   // after a NaN it stays one
       wave_lds_fence();
       T *out = (T *)a.dlogits + (int64_t)row0 * a.dstride;
       asm volatile("" : "+v"(lane));
@@ -685,13 +696,13 @@ __global__ __launch_bounds__(256, SLOTS <= 32 ? 4 : 2) void policy_small_kernel(
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k) {
           const unsigned i = k * 64 + lane;
-          if ((k < LEAST || k < (int)vocab) && i < end) out[i] = (T)all[slot(i)];
+          if ((k < LEAST || k < slots) && i < end) out[i] = (T)all[slot(i)];
         }
       } else {
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k) {
-          const unsigned i = k * 64 + lane, r = __umul24(i, magic) >> 20;
-          if ((k < LEAST || k < (int)vocab) && i < end) out[(int64_t)r * a.dstride + (i - r * vocab)] = (T)all[slot(i)];
+          const unsigned i = k * 64 + lane, r = __umul24(i, magic) >> 22;
+          if ((k < LEAST || k < slots) && i < end) out[(int64_t)r * a.dstride + (i - r * vocab)] = (T)all[slot(i)];
         }
       }
     }
@@ -1046,12 +1057,22 @@ struct Plan {
 // 100 x 131072 bf16 22.0 | 20.1, 128 x 131072 bf16 22.8 | 23.7.
 constexpr size_t kSplitRows = 128, kSplitLoss = 65536, kSplitStats = 98304;   // rows, tokens
 
-Plan plan_of(size_t rows, size_t vocab, bool loss) {
+constexpr size_t kTurnedVocab = 768, kTurnedWork = size_t(1) << 24;   // tokens, elements
+
+Plan plan_of(size_t rows, size_t vocab, bool loss, bool wide) {   // wide: f32
   Plan p;
   if (vocab <= kGroupVocab) {
-    p.route = vocab <= (loss ? kSmallVocab : kSmallStats) ? kSmall : kGroup;
-    if (p.route == kGroup)
-      while (32u << p.lanes_log2 < vocab) ++p.lanes_log2;
+    unsigned lanes = 1;
+    while (32 * lanes < vocab) lanes *= 2;
+    // Rows whose vectors of 8 the lanes of policy_group_kernel share out evenly are its own; others are cheaper turned, for 16 bits up to 128
+    // tokens only (a lane reads less at a time there).  us for 2^25 elements, in groups | turned: objective f32 x 64 75 | 59, x 100 94 | 64,
+    // x 128 61 | 58, x 151 77 | 61, x 192 57 | 72, x 600 62 | 61, bf16 x 64 62 | 49, x 100 74 | 58, x 128 35 | 50, x 151 52 | 53,
+    // x 300 47 | 53; statistics f32 x 64 31 | 30, x 100 35 | 32, x 151 37 | 31, x 256 25 | 29, x 600 37 | 30, bf16 x 64 17 | 21,
+    // x 100 22 | 26, x 151 24 | 24.  For 2^22 elements: objective f32 x 100 16.8 | 16.6, x 151 15.6 | 16.8, for 2^20 10.2 | 10.8, 9.6 | 11.8.
+    const bool even = vocab % (8 * lanes) == 0;
+    const bool turned = vocab <= 48 || (loss && vocab <= 64) || (!even && vocab <= (wide ? kTurnedVocab : loss ? 128 : 0) && rows >= kTurnedWork / vocab);
+    p.route = turned ? kSmall : kGroup;
+    while ((turned ? 48u : 32u) << p.lanes_log2 < vocab) ++p.lanes_log2;
     const size_t per = 256u >> p.lanes_log2;
     p.blocks = (unsigned)std::min<size_t>((rows + per - 1) / per, kGroupBlocks);
   } else if (rows < kSplitRows && vocab > (loss ? kSplitLoss : kSplitStats)) {
@@ -1080,21 +1101,27 @@ void launch_group(const Plan &p, const PolicyArgs &a, hipStream_t s) {
     else hipLaunchKernelGGL((policy_group_kernel<T, LOSS, 4>), grid, block, 0, s, a, p.lanes_log2);
     return;
   }
-  const unsigned magic = ((1u << 20) + a.vocab - 1) / a.vocab;       // exact for the 64 * vocab elements of a wave's rows
-  switch (a.vocab <= 32 ? (a.vocab + 3) / 4 : (a.vocab + 7) / 8 * 2) {
-    case 1: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 4>), grid, block, 0, s, a, magic); break;
-    case 2: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 8>), grid, block, 0, s, a, magic); break;
-    case 3: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 12>), grid, block, 0, s, a, magic); break;
-    case 4: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 16>), grid, block, 0, s, a, magic); break;
-    case 5: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 20>), grid, block, 0, s, a, magic); break;
-    case 6: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 24>), grid, block, 0, s, a, magic); break;
-    case 7: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 28>), grid, block, 0, s, a, magic); break;
-    case 8: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 32>), grid, block, 0, s, a, magic); break;
-    case 10: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 40>), grid, block, 0, s, a, magic); break;
-    case 12: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 48>), grid, block, 0, s, a, magic); break;
-    case 14: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 56>), grid, block, 0, s, a, magic); break;
-    default:
-      if constexpr (LOSS) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 64>), grid, block, 0, s, a, magic);
+  const unsigned magic = ((1u << 22) + a.vocab - 1) / a.vocab;       // exact for the 64 * 48 elements of a wave, at most, and 768 tokens
+  const unsigned slots = (a.vocab + (1u << p.lanes_log2) - 1) >> p.lanes_log2;
+  if (p.lanes_log2) {
+    if constexpr (LOSS || std::is_same<T, float>::value) {      // see plan_of
+      if (slots <= 32) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 32, true>), grid, block, 0, s, a, magic, p.lanes_log2);
+      else if (slots <= 40) hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 40, true>), grid, block, 0, s, a, magic, p.lanes_log2);
+      else hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 48, true>), grid, block, 0, s, a, magic, p.lanes_log2);
+    }
+    return;
+  }
+  switch (slots <= 32 ? (slots + 3) / 4 : (slots + 7) / 8 * 2) {
+    case 1: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 4, false>), grid, block, 0, s, a, magic, 0); break;
+    case 2: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 8, false>), grid, block, 0, s, a, magic, 0); break;
+    case 3: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 12, false>), grid, block, 0, s, a, magic, 0); break;
+    case 4: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 16, false>), grid, block, 0, s, a, magic, 0); break;
+    case 5: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 20, false>), grid, block, 0, s, a, magic, 0); break;
+    case 6: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 24, false>), grid, block, 0, s, a, magic, 0); break;
+    case 7: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 28, false>), grid, block, 0, s, a, magic, 0); break;
+    case 8: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 32, false>), grid, block, 0, s, a, magic, 0); break;
+    case 10: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 40, false>), grid, block, 0, s, a, magic, 0); break;
+    default: hipLaunchKernelGGL((policy_small_kernel<T, LOSS, 48, false>), grid, block, 0, s, a, magic, 0);
   }
 }
 
@@ -1187,7 +1214,7 @@ int ppo_xp_shape_logits_backward(int device, void *stream, int dtype, const void
 }
 
 size_t ppo_xp_policy_workspace(size_t rows, size_t vocab, int loss) {
-  return rows && vocab ? plan_of(rows, vocab, loss != 0).bytes : 0;
+  return rows && vocab ? std::max(plan_of(rows, vocab, loss != 0, false).bytes, plan_of(rows, vocab, loss != 0, true).bytes) : 0;
 }
 
 int ppo_xp_action_stats(int device, void *stream, int dtype, const void *logits, int64_t logits_stride, const int64_t *actions,
@@ -1196,7 +1223,7 @@ int ppo_xp_action_stats(int device, void *stream, int dtype, const void *logits,
   if (rows == 0 || vocab == 0) return 0;
   if (!actions || !neglogps || !entropies) return ppoxp_fail(PPO_XP_EINVAL, "action_stats: NULL argument");
   if (rows > kMaxGrid) return ppoxp_fail(PPO_XP_EINVAL, "action_stats: %zu rows are too many for one launch", rows);
-  const Plan p = plan_of(rows, vocab, false);
+  const Plan p = plan_of(rows, vocab, false, dtype == PPO_XP_F32);
   if (int rc = check_workspace("action_stats", p, workspace, workspace_bytes)) return rc;
   PolicyArgs a{};
   a.logits = logits; a.stride = logits_stride; a.actions = actions; a.neglogps = neglogps; a.entropies = entropies;
@@ -1227,7 +1254,7 @@ int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, 
       !entropies || !stats)
     return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: NULL argument");
   if (rows > kMaxGrid) return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: %zu rows are too many for one launch", rows);
-  const Plan p = plan_of(rows, vocab, true);
+  const Plan p = plan_of(rows, vocab, true, dtype == PPO_XP_F32);
   if (int rc = check_workspace("policy_loss", p, workspace, workspace_bytes)) return rc;
   PolicyArgs a{};
   a.logits = logits; a.stride = logits_stride; a.actions = b->actions; a.neglogps = neglogps; a.entropies = entropies;

@@ -290,7 +290,8 @@ def softmax64(logits, actions):
 
 POLICY = [(1, 1), (1, 2), (3, 3), (300, 6), (257, 18), (130, 63), (131, 64), (129, 65), (70, 151), (33, 512), (17, 513), (9, 1000),
           (5, 2048), (6, 2049), (5, 4099), (4, 8192), (3, 8193), (3, 16385), (2, 32768), (2, 50001), (3, 65537), (2, 131072), (2, 131075),
-          (1, 200003), (1000, 33), (130, 40), (129, 41), (77, 48), (99, 49), (66, 56), (65, 57), (450, 25)]
+          (1, 200003), (1000, 33), (130, 40), (129, 41), (77, 48), (99, 49), (66, 56), (65, 57), (450, 25), (67, 97), (91, 100), (45, 129), (130, 150),
+          (29, 193), (23, 385), (50, 386), (21, 600), (19, 768), (18, 767), (17, 769)]
 
 
 def policy_inputs(R, V, dtype, seed, padded=False):

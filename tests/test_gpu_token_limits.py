@@ -11,7 +11,9 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("R,V,dtype", [(20000, 2100, BF16), (8193, 2049, F32), (40000, 40, F16), (70001, 5, F32), (3, 300001, BF16), (127, 66000, F16),
-                                       (128, 66000, F16), (130, 140001, BF16)])
+                                       (128, 66000, F16), (130, 140001, BF16),
+                                       (260111, 65, F32), (173000, 97, F32), (168001, 100, BF16), (111200, 151, F32), (43800, 385, F32),
+                                       (21900, 767, F32)])
 def test_loss_routes_with_many_records(R, V, dtype):
     """Sums over several slices (more than 8192 records), workgroups that walk over rows, split rows, rows beyond the registers."""
     import ppo_amd
@@ -30,6 +32,35 @@ def test_loss_routes_with_many_records(R, V, dtype):
         assert torch.equal(r2.stats, r.stats) and torch.equal(r2.dlogits, r.dlogits)
     nlp, ent = ppo_amd.action_stats(logits, a)
     assert torch.all(((nlp.double() - w["nlp"]).abs() <= w["err_nlp"])[real]) and torch.all(((ent.double() - w["ent"]).abs() <= w["err_ent"])[real])
+
+
+@pytest.mark.parametrize("R,V,dtype", [(1001, 50, F32), (1001, 63, BF16), (258200, 65, F32), (168001, 100, F16), (111200, 150, F32), (87000, 193, F32),
+                                       (43700, 386, F32), (22003, 763, F32)])
+def test_rows_apart_give_the_same_bits(R, V, dtype):
+    """Large calls over rows that lie apart, at odd addresses: only the addresses differ, nothing beside the rows is written."""
+    import ppo_amd
+    g, x, a = policy_inputs(R, V, dtype, R, padded=True)
+    x[5, ::2] = -math.inf
+    x[6] = -math.inf
+    x[7, V - 1] = math.nan
+    b = batch_of(g, torch.where(torch.isfinite(x), x, 0.0), a)
+    wide = torch.full((R, V + 3), 5.0, dtype=dtype, device="cuda")
+    wide[:, 1:V + 1] = x
+    out = torch.full((R, V + 2), 7.0, dtype=dtype, device="cuda")
+    r = ppo_amd.policy_loss(x, b.new_values, b)
+    q = ppo_amd.policy_loss(wide[:, 1:V + 1], b.new_values, b, out=out[:, 1:V + 1])
+    same = lambda p, t: torch.equal(p.nan_to_num(1e30), t.nan_to_num(1e30))  # noqa: E731
+    assert same(q.dlogits.float(), r.dlogits.float()) and same(q.neglogps, r.neglogps) and same(q.entropies, r.entropies)
+    assert torch.equal(q.dvalues, r.dvalues)
+    assert torch.all(out[:, 0] == 7) and torch.all(out[:, V + 1:] == 7) and torch.all(wide[:, 0] == 5) and torch.all(wide[:, V + 1:] == 5)
+    pad = a < 0
+    assert torch.all(r.dlogits[pad] == 0) and torch.all(r.neglogps[pad] == 0) and torch.all(r.dvalues[pad] == 0)
+    if not pad[6]:
+        assert torch.all(r.dlogits[6] == 0) and r.neglogps[6] == math.inf
+    assert torch.all(r.dlogits[7].isnan()) if not pad[7] else torch.all(r.dlogits[7] == 0)
+    if dtype == F32:          # statistics of 16-bit rows this long begin at the row's 4-byte boundary: which lane adds what follows the address
+        for p, t in zip(ppo_amd.action_stats(wide[:, 1:V + 1], a), ppo_amd.action_stats(x, a)):
+            assert same(p, t)
 
 
 @pytest.mark.parametrize("offset,spread", [(0.0, 30.0), (80.0, 1.0), (-3000.0, 2.0), (5000.0, 2.0), (60000.0, 100.0), (-1e9, 1.0), (3e37, 1e36)])
