@@ -712,7 +712,8 @@ __global__ __launch_bounds__(256, SLOTS <= 32 ? 4 : 2) void policy_small_kernel(
 }
 
 // Up to kGroupVocab tokens: `lanes` neighbouring lanes hold one row, NV vectors of 8 each, and a wave as many rows as it can: what a
-// row costs beside its elements (some 200 instructions) is paid once a wave.
+// row costs beside its elements (some 200 instructions) is paid once a wave.  Memory bounds it where rows fill their lanes (objective of
+// 131072 x 256 f32 277 MB in 60 us, bf16 143 MB in 33 us), the row's cost and its odd ends where they do not (222214 x 151 bf16 52 us).
 constexpr unsigned kGroupVocab = 2048;
 
 template <typename T, bool LOSS, int NV>
@@ -779,7 +780,8 @@ __global__ __launch_bounds__(THREADS) void policy_stats_row_kernel(PolicyArgs a)
 }
 
 // One workgroup per row, the whole row in registers (NV vectors of 8 a thread): read once, the gradient written from there.
-// Rows of up to half the registers leave room for a second workgroup, which loads while the first computes.
+// Rows of up to half the registers leave room for a second workgroup, which loads while the first computes.  4096 x 50001 bf16 with
+// padding rows: 148 us, 761 MB; the vector unit is busy for 68 % of it, two powers an element.
 template <typename T, int NV>
 __global__ __launch_bounds__(1024, NV * sizeof(Raw8<T>) <= 128 ? 8 : 4) void policy_loss_row_kernel(PolicyArgs a) {
   __shared__ Softmax red[16];
@@ -805,7 +807,8 @@ __global__ __launch_bounds__(1024, NV * sizeof(Raw8<T>) <= 128 ? 8 : 4) void pol
   write_gradient<NV>(r, k, (T *)a.dlogits + (int64_t)row * a.dstride - at.first, tid, threads, at, action + at.first, plain);
 }
 
-// Rows too long for the registers of a workgroup: read a second time for the gradient, out of the caches as far as they hold it.
+// Rows too long for the registers of a workgroup: read a second time for the gradient, out of the caches as far as they hold it
+// (256 x 262144 f32 167 us, 4.8 TB/s with the second read; bf16 75 us).
 template <typename T>
 __global__ __launch_bounds__(1024) void policy_loss_long_kernel(PolicyArgs a) {
   __shared__ Softmax red[16];
