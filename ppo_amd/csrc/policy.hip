@@ -177,8 +177,9 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
       const int64_t h = r.hist_row ? r.hist_row[row] : (int64_t)row;
       if (h < 0 || h >= r.hist_rows) continue;
       const int end = (int)min(r.hist_end ? (int64_t)r.hist_end[row] : r.hist_len, r.hist_len);
-      const int begin = r.hist_begin ? max(r.hist_begin[row], 0) : 0;
-      const int gen = r.gen_begin ? r.gen_begin[row] : begin;
+      // 64 bits: a first position near the type's end plus the thread's own must not wrap round to in front of the history
+      const int64_t begin = r.hist_begin ? min((int64_t)max(r.hist_begin[row], 0), r.hist_len) : 0;
+      const int64_t gen = r.gen_begin ? r.gen_begin[row] : begin;
       const int64_t base = h * r.hist_row_stride;
       const T *logits = MODE == kGather ? (const T *)a.logits + (int64_t)row * a.logits_stride : nullptr;
       float up = 0.f, down = 0.f;                    // backward: the slope at positive logits and at others
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
         down = q.rep * q.inv_t;
       }
       constexpr int kTokens = 8;                     // on their way at a time
-      for (int64_t k0 = begin + (int)(MULTI ? tid & (lanes - 1) : tid); k0 < end; k0 += kTokens * lanes) {
+      for (int64_t k0 = begin + (MULTI ? tid & (lanes - 1) : tid); k0 < end; k0 += kTokens * lanes) {
         int64_t tok[kTokens];
 #pragma unroll
         for (int j = 0; j < kTokens; ++j) {

@@ -1,0 +1,36 @@
+"""Arguments of the logit rules and the objective at the ends of their types' ranges."""
+import pytest
+import torch
+
+from test_gpu_policy_ops import BF16, F16, F32, check_shape, gen, half, randn, rules64
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+LAST, FIRST = 2 ** 31 - 1, -2 ** 31
+
+# short rows that share a workgroup, a workgroup a row with few and with many chunks; histories short and long for their vocabulary
+ROUTES = [(12, 50, 40), (12, 50, 2), (12, 5000, 40), (12, 5000, 700), (96, 20011, 40), (96, 20011, 900), (520, 3000, 90)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("R,V,L", ROUTES)
+def test_history_positions_at_the_ends_of_32_bits(R, V, L, dtype):
+    """Positions are clamped to the history: a begin far behind it leaves nothing, an end far behind it all of it."""
+    import ppo_amd
+    g = gen(R + V + L)
+    x = (randn(g, R, V) * 2).to(dtype)
+    hist = torch.randint(0, V, (R, L), generator=g, device="cuda")
+    i32 = lambda *v: torch.tensor([v[k % len(v)] for k in range(R)], dtype=torch.int64, device="cuda").int()  # noqa: E731
+    kw = dict(history=hist, repetition=1.5, presence=0.25, frequency=0.5, temperature=0.75,
+              hist_begin=i32(LAST, 0, FIRST, LAST - 255, L, LAST - 1, L - 1, 1),
+              hist_end=i32(LAST, L, LAST, L + 1, FIRST, 0, LAST - 3),
+              gen_begin=i32(0, LAST, FIRST, L, LAST - 7))
+    check_shape(x, ppo_amd.shape_logits(x, **kw), kw)
+    grad = randn(g, R, V).to(dtype)
+    bk = {k: v for k, v in kw.items() if k not in ("presence", "frequency", "gen_begin")}
+    got = ppo_amd.shape_logits_backward(grad, x, **bk).cpu().double()
+    seen, _, _, rep, _, _, temp = rules64(x, kw, V)
+    d = grad.cpu().double()
+    want = torch.where(seen, torch.where(x.cpu().double() > 0, d / rep, d * rep), d) / temp
+    # 1 / T, 1 / rep, their product and the product with it, then the rounding to the type
+    assert torch.all((got - want).abs() <= (half(dtype) + 4 * U) * want.abs() * (1 + half(dtype)) + 2.0 ** -25 * (dtype == F16))
