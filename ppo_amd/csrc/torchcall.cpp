@@ -308,6 +308,9 @@ Store store_of(PyObject *const *a) {
       s.scales.scalar_type() != at::kFloat || s.codes.size(1) != bytes || s.scales.size(1) != (s.width + s.group - 1) / s.group ||
       s.codes.size(0) != s.scales.size(0) || (s.codes.size(1) > 1 && s.codes.stride(1) != 1) || (s.scales.size(1) > 1 && s.scales.stride(1) != 1))
     panic("QuantizedRows: codes and scales no longer have the shapes they were made with");
+  // rows that share storage (expanded ones, say) would be addressed as if they lay apart, beyond its end
+  if (s.codes.size(0) > 1 && (s.codes.stride(0) < s.codes.size(1) || s.scales.stride(0) < s.scales.size(1)))
+    panic("QuantizedRows: rows of codes and scales must not overlap");
   s.codes_stride = std::max<int64_t>(s.codes.stride(0), s.codes.size(1));
   s.scales_stride = std::max<int64_t>(s.scales.stride(0), s.scales.size(1));
   return s;

@@ -1,0 +1,32 @@
+"""A QuantizedRows whose attributes were exchanged, and rows written and read in calls of every size."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def refused(store, rows):
+    from ppo_amd import PpoXpPanic
+    index = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for call in (lambda: store.write(rows), lambda: store.read(), lambda: store.read(index), lambda: store.read(slice(0, 1))):
+        with pytest.raises(PpoXpPanic):
+            call()
+
+
+def test_refuses_stores_whose_rows_overlap():
+    """Exchanged tensors of the right shape whose rows share storage: expanded ones, windows that move by less than a row."""
+    import ppo_amd
+    x = torch.zeros(8, 64, device="cuda")
+    good = ppo_amd.QuantizedRows(8, 64, "int8", 32)
+    overlapping = [(good.codes[:1].expand(8, 64), good.scales), (good.codes, good.scales[:1].expand(8, 2)),
+                   (torch.zeros(200, dtype=torch.int8, device="cuda").as_strided((8, 64), (16, 1)), good.scales),
+                   (good.codes, torch.zeros(9, device="cuda").as_strided((8, 2), (1, 1)))]
+    for codes, scales in overlapping:
+        s = ppo_amd.QuantizedRows.of(good.codes, good.scales, 64, "int8", 32)
+        s.codes, s.scales = codes, scales
+        refused(s, x)
+    # one row has no distance to the next: any stride is good
+    s = ppo_amd.QuantizedRows.of(good.codes[:1], good.scales[:1], 64, "int8", 32)
+    s.codes, s.scales = good.codes[:1].as_strided((1, 64), (0, 1)), good.scales[:1].as_strided((1, 2), (0, 1))
+    s.write(x[:1] + 2.0)
+    assert torch.all(s.read() == 2.0)
