@@ -303,6 +303,7 @@ struct Store {
 // codes, scales, row size, PPO_XP_Q_*, group.  QuantizedRows has checked them once; its tensors may have been exchanged since.
 Store store_of(PyObject *const *a) {
   Store s{some(a[0], "codes"), some(a[1], "scales"), whole(a[2]), whole(a[3]), whole(a[4]), 0, 0};
+  if (s.group < 1) panic("QuantizedRows: group " + num(s.group) + " is not positive");
   const int64_t bytes = s.kind == PPO_XP_Q_INT4 ? (s.width + 1) / 2 : s.width;
   if (!s.codes.is_cuda() || s.codes.device() != s.scales.device() || s.codes.dim() != 2 || s.scales.dim() != 2 || s.codes.element_size() != 1 ||
       s.scales.scalar_type() != at::kFloat || s.codes.size(1) != bytes || s.scales.size(1) != (s.width + s.group - 1) / s.group ||

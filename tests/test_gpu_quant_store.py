@@ -30,3 +30,14 @@ def test_refuses_stores_whose_rows_overlap():
     s.codes, s.scales = good.codes[:1].as_strided((1, 64), (0, 1)), good.scales[:1].as_strided((1, 2), (0, 1))
     s.write(x[:1] + 2.0)
     assert torch.all(s.read() == 2.0)
+
+
+def test_refuses_a_changed_group():
+    """The attributes that describe the store are looked at with each call as well."""
+    import ppo_amd
+    x = torch.zeros(8, 64, device="cuda")
+    for name, values in (("group", (0, -1, -64, 33, 1 << 40)), ("row_size", (0, -1, 63, 1 << 40)), ("_kind", (0, 4, 3))):
+        for value in values:
+            s = ppo_amd.QuantizedRows(8, 64, "int8", 32)
+            setattr(s, name, value)
+            refused(s, x)
