@@ -112,25 +112,41 @@ class ExperienceBuffer:
     def new_quantized(cls, num_envs, row_size, capacity, format="int8", group=64, dtype=None, gamma=0.99, lam=0.95, device=0):
         """A buffer whose observation rows (hidden states of `row_size` elements, f32 / bf16 / f16) are kept in 8 or 4 bits: quantised as
         add_experience* writes them, read back as `dtype` (default f32) by the minibatches of a pass (quant.QuantizedRows).  The
-        other streams and the pass itself are the ordinary ones; rows are written and read on torch's current stream, a minibatch's
-        when the iterator yields it: insert again only after that (as with streaming passes)."""
+        other streams and the pass itself are the ordinary ones; a minibatch's rows are read when the iterator yields it: insert again
+        only after that (as with streaming passes).  Inserts and reads may run on different torch streams."""
         import torch
         from .quant import QuantizedRows
         self = cls(num_envs, 1, capacity, gamma, lam, device)      # the handle's own rows: one unused float
-        self.rows = QuantizedRows(self.capacity * self.num_envs, row_size, format, group, device)
         self.rows_dtype = torch.float32 if dtype is None else dtype
-        self._no_obs = torch.zeros(self.num_envs, 1, device=self.rows.codes.device)
+        self.rows = self._on_rows(lambda: QuantizedRows(self.capacity * self.num_envs, row_size, format, group, device))
+        self._no_obs = self._on_rows(lambda: torch.zeros(self.num_envs, 1, device=self.rows.codes.device))
         return self
+
+    def _on_rows(self, call):
+        """`call`, which writes or reads quantised rows on torch's current stream, behind everything the handle's stream holds and
+        before everything it is given next: inserts and reads are in order through it whichever torch streams they run on."""
+        cur, hs = self._order_streams()
+        if hs is not None:
+            cur.wait_stream(hs)
+        out = call()
+        if hs is not None:
+            hs.wait_stream(cur)
+        return out
 
     def _write_rows(self, obs, steps):
         """Quantises the rows of `steps` steps that are about to be inserted at the ring's next places ([steps * N, row_size])."""
-        n, cap = self.num_envs, self.capacity
-        done, at = max(0, steps - cap), self.counter                # what a later step of this call overwrites is not written
-        while done < steps:
-            place = (at + done) % cap
-            run = min(steps - done, cap - place)
-            self.rows.write(obs[done * n:(done + run) * n], place * n)
-            done += run
+        def write():
+            n, cap = self.num_envs, self.capacity
+            done, at = max(0, steps - cap), self.counter            # what a later step of this call overwrites is not written
+            while done < steps:
+                place = (at + done) % cap
+                run = min(steps - done, cap - place)
+                self.rows.write(obs[done * n:(done + run) * n], place * n)
+                done += run
+        self._on_rows(write)
+
+    def _read_all_rows(self, n):
+        return self._on_rows(lambda: self.rows.read(slice(0, n), dtype=self.rows_dtype))
 
     def _device_rows(self, obs, steps):
         import torch
@@ -269,7 +285,7 @@ class ExperienceBuffer:
         M, D, d = v.num_steps, self.obs_size, self.device
         self.sync()
         if self.rows is not None:
-            obs = self.rows.read(slice(0, M), dtype=self.rows_dtype)     # a copy: the rows as they read back
+            obs = self._read_all_rows(M)                                 # a copy: the rows as they read back
             obs._ppo_owner = self
         else:
             obs = device_tensor(v.observations, (M, D), torch.float32, d, self)
@@ -319,7 +335,7 @@ class ExperienceBuffer:
         import torch
         v = self._views()
         if name == "observations" and self.rows is not None:
-            return self.rows.read(slice(0, v.num_steps), dtype=self.rows_dtype)
+            return self._read_all_rows(v.num_steps)
         dt = torch.int64 if name == "actions" else torch.float32
         shape = (v.num_steps, self.obs_size) if name == "observations" else (v.num_steps,)
         self.sync()

@@ -132,11 +132,6 @@ class ExperienceBatcherIterator:
             if hs is not None:
                 cur.wait_stream(hs)
             buf._pass_perm = None
-        if buf.rows is not None:
-            # reads of quantised rows on torch's stream may still be using the previous pass's permutation
-            cur, hs = buf._order_streams()
-            if hs is not None:
-                hs.wait_stream(cur)
         if perm is not None and hasattr(perm, "is_cuda") and perm.is_cuda:
             import torch
             if perm.numel() != len(batcher) or perm.dtype not in (torch.int32,) or not perm.is_contiguous():
@@ -211,12 +206,9 @@ class ExperienceBatcherIterator:
         ptr = L.ppo_xp_pass_perm_device(buf.handle)      # a keyed bijection is written out on the handle's stream the first time
         if not ptr:
             check(_lib.ESTATE)
-        cur, hs = buf._order_streams()
-        if hs is not None:
-            cur.wait_stream(hs)
         start = min(k * B, M - B)
         index = device_tensor(ptr, (M,), torch.uint32, buf.device, buf)[start:start + B]
-        return buf.rows.read(index, dtype=buf.rows_dtype)
+        return buf._on_rows(lambda: buf.rows.read(index, dtype=buf.rows_dtype))      # ... and the next pass's behind this read of it
 
     def next_host(self, out: "HostBatch | None" = None) -> "HostBatch | None":
         """Iterator::next as the reference's caller sees it (data.rs:166-182 feeds six host Vecs to
