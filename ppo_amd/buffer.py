@@ -148,15 +148,16 @@ class ExperienceBuffer:
     def _read_all_rows(self, n):
         return self._on_rows(lambda: self.rows.read(slice(0, n), dtype=self.rows_dtype))
 
-    def _device_rows(self, obs, steps):
+    def _device_rows(self, obs, *steps):
+        """`obs` [*steps, NUM_ENVS, row_size], from the host or a device, as rows on the store's device."""
         import torch
         t = torch.as_tensor(np.asarray(obs)) if not isinstance(obs, torch.Tensor) else obs
+        want = (*steps, self.num_envs, self.rows.row_size)
+        if tuple(t.shape) != want:
+            raise PpoXpPanic(_lib.EINVAL, f"add_experience: obs must be {list(want)}, not {list(t.shape)} (reference panics, buffer.rs:97-112)")
         if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             t = t.to(torch.float32)
-        t = t.to(self.rows.codes.device)
-        if t.numel() != steps * self.num_envs * self.rows.row_size:
-            raise PpoXpPanic(_lib.EINVAL, f"add_experience: obs must be [NUM_ENVS, {self.rows.row_size}] a step (reference panics, buffer.rs:97-112)")
-        return t.reshape(steps * self.num_envs, self.rows.row_size)
+        return t.to(self.rows.codes.device).reshape(-1, self.rows.row_size)
 
     def close(self):
         if getattr(self, "_h", None) and self._h.value:
@@ -180,7 +181,7 @@ class ExperienceBuffer:
     def add_experience(self, obs, rewards, actions, vals, dones, neglogps):
         """buffer.rs:84-121.  obs [NUM_ENVS, OBS_SIZE]; the rest [NUM_ENVS]; dones are bools."""
         if self.rows is not None:
-            states, obs = self._device_rows(obs, 1), np.zeros((self.num_envs, 1), np.float32)
+            states, obs = self._device_rows(obs), np.zeros((self.num_envs, 1), np.float32)
         obs = _np(obs, np.float32, "obs")
         rewards, vals, neglogps = (_np(x, np.float32, n) for x, n in ((rewards, "rewards"), (vals, "vals"), (neglogps, "neglogps")))
         actions = _np(actions, np.uint64, "actions")
