@@ -98,9 +98,12 @@ at::Tensor result(PyObject *o, const at::Tensor &like, const char *what, Matrix 
   return out;
 }
 
-// A caller's `out` changes under autograd's eyes: what was saved of it for a backward pass is known to be stale.
+// A caller's tensor changes under autograd's eyes: what was saved of it for a backward pass is known to be stale.
+void changed(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 void written(PyObject *o, const at::Tensor &out) {
-  if (o != Py_None && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+  if (o != Py_None) changed(out);
 }
 
 void *stream_of(int device) {
@@ -323,6 +326,8 @@ PyObject *write(PyObject *const *a) {                       // store, rows, at
   const int64_t at = whole(a[6]);
   if (m.cols != s.width || m.device != s.codes.get_device() || at < 0)
     panic("write: rows of " + num(s.width) + " on cuda:" + num(s.codes.get_device()) + " and at >= 0 expected");
+  changed(s.codes);
+  changed(s.scales);
   done(launch(g_quantize, m.device, stream_of(m.device), m.dtype, m.p, m.stride, m.rows, m.cols, (int)s.kind, s.group, s.codes.data_ptr(), s.codes_stride,
                   s.scales.data_ptr<float>(), s.scales_stride, s.codes.size(0), at));
   Py_RETURN_NONE;
@@ -356,6 +361,7 @@ PyObject *read(PyObject *const *a) {                        // store, index or N
       panic(std::string("read: out must be ") + at::toString(type) + " [" + num(n) + ", " + num(s.width) + "] on the store's device");
   }
   const Matrix o = matrix(out, "read");
+  written(a[9], out);
   done(launch(g_dequantize, device, stream_of(device), (int)dt, s.codes.data_ptr(), s.codes_stride, s.scales.data_ptr<float>(), s.scales_stride, s.codes.size(0),
                     s.width, (int)s.kind, s.group, index, bits, first, n, o.p, o.stride));
   return THPVariable_Wrap(out);

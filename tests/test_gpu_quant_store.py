@@ -41,3 +41,37 @@ def test_refuses_a_changed_group():
             s = ppo_amd.QuantizedRows(8, 64, "int8", 32)
             setattr(s, name, value)
             refused(s, x)
+
+
+def test_rows_written_in_place_are_seen_by_autograd():
+    """What a backward pass saved of a tensor that read or write then fills is known to be stale."""
+    import ppo_amd
+    store = ppo_amd.QuantizedRows(8, 64, "int8", 32)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    store.write(torch.randn(8, 64, generator=g, device="cuda"))
+    index = torch.arange(4, device="cuda").int()
+    w = torch.randn(64, 3, generator=g, device="cuda", requires_grad=True)
+    out = torch.empty(4, 64, device="cuda")
+    y = store.read(index, out=out)
+    assert y is out
+    loss = (y @ w).sum()                                   # saves y for the gradient of w
+    store.read(index + 4, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    loss = (store.read(index, out=out) @ w).sum()
+    store.read(index + 4)                                  # a new tensor: what was saved stays good
+    loss.backward()
+    v = torch.randn(8, 2, generator=g, device="cuda", requires_grad=True)
+    loss = (v * store.scales).sum()                        # saves the scales
+    store.write(torch.ones(8, 64, device="cuda"))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    before = store.codes._version
+    store.write(torch.ones(1, 64, device="cuda"), 3)
+    assert store.codes._version > before
+    with torch.inference_mode():
+        out = torch.empty(4, 64, device="cuda")
+        assert torch.equal(store.read(index, out=out), store.read(index))
+        s = ppo_amd.QuantizedRows(8, 64, "int8", 32)
+        s.write(torch.ones(8, 64, device="cuda"))
