@@ -363,7 +363,8 @@ typedef struct ppo_xp_logit_rules {
   int64_t mask_stride;              /* in words / bytes; 0: one mask row for all                                                */
   int64_t mask_rows;                /* mask rows                                                                                */
   const int32_t *mask_row;          /* [rows] mask row of each logits row (NULL: the row itself); one outside 0..mask_rows = unconstrained */
-  float repetition, presence, frequency, temperature;  /* scalars: 1, 0, 0, 1 change nothing; repetition and temperature > 0    */
+  float repetition, presence, frequency, temperature;  /* scalars: 1, 0, 0, 1 change nothing; finite, repetition and temperature at
+                                       least 2^-126 (a row's own value below that counts as 2^-126)                             */
   int32_t history_bits;             /* 32 or 64                                                                                 */
   int32_t mask_kind;                /* PPO_XP_MASK_*                                                                            */
 } ppo_xp_logit_rules;

@@ -43,13 +43,18 @@ struct RowRules {
   const uint8_t *mask;
 };
 
+// Divisors from the least normal number on have a finite reciprocal (of smaller ones it is infinite, and 0 times that NaN): a
+// row's own value below it counts as that number, a scalar was refused.
+constexpr float kLeastDivisor = 0x1p-126f;
+__device__ __forceinline__ float divisor(float x) { return x < kLeastDivisor ? kLeastDivisor : x; }   // NaN stays NaN
+
 __device__ __forceinline__ RowRules row_rules(const ppo_xp_logit_rules &r, size_t row) {
   RowRules q;
-  q.rep = r.repetition_rows ? r.repetition_rows[row] : r.repetition;
+  q.rep = divisor(r.repetition_rows ? r.repetition_rows[row] : r.repetition);
   q.inv_rep = 1.f / q.rep;
   q.pres = r.presence_rows ? r.presence_rows[row] : r.presence;
   q.freq = r.frequency_rows ? r.frequency_rows[row] : r.frequency;
-  q.inv_t = 1.f / (r.temperature_rows ? r.temperature_rows[row] : r.temperature);
+  q.inv_t = 1.f / divisor(r.temperature_rows ? r.temperature_rows[row] : r.temperature);
   q.bias = r.bias ? r.bias + (int64_t)row * r.bias_stride : nullptr;
   q.mask = nullptr;
   if (r.mask_kind != PPO_XP_MASK_NONE) {
@@ -950,7 +955,7 @@ __global__ __launch_bounds__(960) void policy_stats_kernel(const double *partial
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
 
-bool finite_positive(float x) { return x > 0.f && std::isfinite(x); }
+bool is_divisor(float x) { return x >= kLeastDivisor && std::isfinite(x); }
 
 int check_rows(const char *who, int dtype, const void *p, int64_t stride, size_t rows, size_t vocab) {
   if (!is_dtype(dtype)) return ppoxp_fail(PPO_XP_EINVAL, "%s: unknown element type %d", who, dtype);
@@ -963,8 +968,8 @@ int check_rows(const char *who, int dtype, const void *p, int64_t stride, size_t
 
 int check_rules(const char *who, const ppo_xp_logit_rules *r, size_t rows, size_t vocab) {
   if (!r) return ppoxp_fail(PPO_XP_EINVAL, "%s: rules is NULL", who);
-  if (!finite_positive(r->repetition) || !finite_positive(r->temperature))
-    return ppoxp_fail(PPO_XP_EINVAL, "%s: repetition %g and temperature %g must be finite and > 0", who, r->repetition, r->temperature);
+  if (!is_divisor(r->repetition) || !is_divisor(r->temperature))
+    return ppoxp_fail(PPO_XP_EINVAL, "%s: repetition %g and temperature %g must be finite and at least 2^-126", who, r->repetition, r->temperature);
   if (!std::isfinite(r->presence) || !std::isfinite(r->frequency))
     return ppoxp_fail(PPO_XP_EINVAL, "%s: presence %g and frequency %g must be finite", who, r->presence, r->frequency);
   if (r->history) {

@@ -24,7 +24,7 @@ def shape_logits(logits, *, history=None, hist_row=None, hist_begin=None, gen_be
     history [H, L] int64 / int32 token ids of any strides - a buffer's actions column is
     `buffer.stream_view("actions").view(T, N).t()` - read at [hist_begin, hist_end) of row hist_row[r] (default: row r, all of it);
     tokens from gen_begin on count for frequency and presence.  repetition, presence, frequency, temperature: a number or one f32
-    per row.  bias f32 [vocab] or [rows, vocab].  mask: bool / uint8 [.., vocab] or int32 words [.., ceil(vocab / 32)], set = allowed,
+    per row; repetition and temperature at least 2^-126 (a number below is refused, a row's own counts as 2^-126).  bias f32 [vocab] or [rows, vocab].  mask: bool / uint8 [.., vocab] or int32 words [.., ceil(vocab / 32)], set = allowed,
     one row for all, one per row, or picked by mask_row (a negative one leaves its row free).  `out` may be `logits`."""
     return _call.shape(logits, history, hist_row, hist_begin, gen_begin, hist_end, repetition, presence, frequency, bias, mask, mask_row,
                        temperature, out)

@@ -34,3 +34,42 @@ def test_history_positions_at_the_ends_of_32_bits(R, V, L, dtype):
     want = torch.where(seen, torch.where(x.cpu().double() > 0, d / rep, d * rep), d) / temp
     # 1 / T, 1 / rep, their product and the product with it, then the rounding to the type
     assert torch.all((got - want).abs() <= (half(dtype) + 4 * U) * want.abs() * (1 + half(dtype)) + 2.0 ** -25 * (dtype == F16))
+
+
+@pytest.mark.parametrize("R,V,L", ROUTES)
+def test_divisors_at_the_ends_of_their_range(R, V, L):
+    """The least and the largest scalars, and rows whose own value lies below the least: those count as the least one."""
+    import ppo_amd
+    g = gen(R + V)
+    x = randn(g, R, V)
+    x[:, ::5] = 0.0                                            # 0 divided by anything is 0
+    x[:, 1::5] *= 2.0 ** -100
+    hist = torch.randint(0, V, (R, L), generator=g, device="cuda")
+    least, most = 2.0 ** -126, float(torch.finfo(F32).max)
+    grad = x.flip(0) * 2.0 ** -30
+    for kw in (dict(temperature=least), dict(repetition=least), dict(temperature=least, repetition=most), dict(temperature=2.0 ** 126), dict(repetition=2.0 ** 126)):
+        kw["history"] = hist
+        seen, _, _, rep, _, _, temp = rules64(x, kw, V)
+        d, l = grad.cpu().double(), x.cpu().double()
+        got, want = ppo_amd.shape_logits(x, **kw).cpu().double(), torch.where(seen, torch.where(l > 0, l / rep, l * rep), l) / temp
+        # The reciprocal of a divisor above 2^126 is a multiple of 2^-149 and at least 2^-128: off by 2^-150 / 2^-128 = 4 u.  Two of
+        # them, two products: 10 u.  A quotient below 2^-126 in between is a multiple of 2^-149 as well, off by 2^-150, which the
+        # division by the temperature magnifies.
+        fits = want.abs() < 2.0 ** 127
+        assert torch.all(((got - want).abs() <= 10 * U * want.abs() + 2.0 ** -150 / temp.clamp(max=1.0) + 2.0 ** -150)[fits]) and not got.isnan().any()
+        slope = torch.where(seen, torch.where(l > 0, 1 / rep, rep), 1.0) / temp
+        got, want = ppo_amd.shape_logits_backward(grad, x, **kw).cpu().double(), d * slope
+        # the slope is one 32-bit number, the product of two reciprocals or of one and the repetition: 4 u + 4 u + u, and the product
+        # with the gradient
+        inside = (slope.abs() < 2.0 ** 127) & (want.abs() < 2.0 ** 127) & (slope.abs() >= 2.0 ** -126)
+        assert torch.all(((got - want).abs() <= 10 * U * want.abs() + 2.0 ** -149)[inside]) and not got[inside].isnan().any()
+    f = lambda *v: torch.tensor([v[k % len(v)] for k in range(R)], dtype=F32, device="cuda")  # noqa: E731
+    below, held = f(0.0, -1.0, 2.0 ** -149, 2.0 ** -128, 2.0 ** -126, 1.0), f(least, least, least, least, least, 1.0)
+    for name in ("temperature", "repetition"):
+        got, want = (ppo_amd.shape_logits(x, history=hist, **{name: v}) for v in (below, held))
+        assert torch.equal(got, want) and not got.isnan().any()
+        got, want = (ppo_amd.shape_logits_backward(grad, x, history=hist, **{name: v}) for v in (below, held))
+        assert torch.equal(got, want) and not got.isnan().any()
+    bad = f(float("nan"), 1.0)
+    got = ppo_amd.shape_logits(x, temperature=bad)
+    assert got[::2].isnan().all() and torch.equal(got[1::2], x[1::2])
