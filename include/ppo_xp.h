@@ -356,7 +356,8 @@ typedef struct ppo_xp_logit_rules {
   const int32_t *hist_begin;        /* [rows] first position (NULL: 0); positions are clamped to 0..hist_len                    */
   const int32_t *gen_begin;         /* [rows] first position that counts for frequency / presence (NULL: begin)                 */
   const int32_t *hist_end;          /* [rows] one past the last position (NULL: hist_len)                                       */
-  const float *repetition_rows, *presence_rows, *frequency_rows, *temperature_rows; /* [rows] per-row values (NULL: the scalars) */
+  const float *repetition_rows, *presence_rows, *frequency_rows, *temperature_rows; /* [rows] per-row values (NULL: the scalars);
+                                       an infinite presence or frequency forbids what it applies to, and nothing else           */
   const float *bias;                /* [rows, vocab] f32, added before the temperature                                          */
   int64_t bias_stride;              /* 0: one bias row for all                                                                  */
   const void *mask;                 /* BITS: u32 words, bit v % 32 of word v / 32 set = allowed; BYTES: one byte per token, non-zero = allowed */

@@ -253,7 +253,7 @@ __global__ __launch_bounds__(256) void shape_logits_kernel(ShapeArgs a) {
           if (!__any(w != 0)) continue;
           const float n = (float)(w & ~kPromptOnly);
           x[i] *= w ? (x[i] > 0.f ? q.inv_rep : q.rep) : 1.f;
-          x[i] -= q.freq * n + (n > 0.f ? q.pres : 0.f);
+          x[i] -= n > 0.f ? q.freq * n + q.pres : 0.f;    // not freq * 0: it may be infinite
         }
       }
       if (!MULTI && q.bias) {

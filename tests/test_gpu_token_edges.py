@@ -73,3 +73,20 @@ def test_divisors_at_the_ends_of_their_range(R, V, L):
     bad = f(float("nan"), 1.0)
     got = ppo_amd.shape_logits(x, temperature=bad)
     assert got[::2].isnan().all() and torch.equal(got[1::2], x[1::2])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("R,V,L", ROUTES)
+def test_an_infinite_penalty_forbids_the_tokens_it_applies_to(R, V, L, dtype):
+    import ppo_amd
+    g = gen(V)
+    x = randn(g, R, V).to(dtype)
+    hist = torch.randint(0, V, (R, L), generator=g, device="cuda")
+    half_way = torch.full((R,), L // 2, dtype=torch.int32, device="cuda")
+    counted = torch.zeros(R, V, device="cuda").scatter_(1, hist[:, L // 2:], 1.0) > 0      # tokens of the prompt only are not counted
+    inf = torch.full((R,), float("inf"), device="cuda")
+    inf[::3] = 0.0
+    for kw in (dict(frequency=inf), dict(presence=inf), dict(frequency=inf, presence=inf)):
+        out = ppo_amd.shape_logits(x, history=hist, gen_begin=half_way, **kw)
+        forbidden = counted & (inf > 0)[:, None]
+        assert torch.all(out[forbidden] == -float("inf")) and torch.equal(out[~forbidden], x[~forbidden])
