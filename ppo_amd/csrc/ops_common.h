@@ -201,7 +201,9 @@ inline int launched(const char *who) {
 
 inline bool is_dtype(int d) { return d == PPO_XP_F32 || d == PPO_XP_BF16 || d == PPO_XP_F16; }
 inline size_t dtype_bytes(int d) { return d == PPO_XP_F32 ? 4 : 2; }
-constexpr size_t kMaxGrid = 0x7fffffff;
+// A dispatch counts its work items in 32 bits, and more of them wrap round without an error: 2^24 + 8 workgroups of 256 ran as 8.
+inline bool one_launch(size_t workgroups, size_t threads) { return workgroups <= size_t(0xffffffff) / threads; }
+constexpr size_t kMaxRows = 0x7fffffff;
 constexpr size_t kMaxVocab = size_t(1) << 30;
 
 }  // namespace ppoxp_ops

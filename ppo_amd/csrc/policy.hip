@@ -1033,14 +1033,15 @@ int shape(const char *who, int device, void *stream, int dtype, ShapeArgs &a, si
   // workgroups go to the 8 XCDs in turn, and of an even number of chunks a short last one is always the same XCDs': equal parts then
   // (4096 x 10000 f32 with a history, 8192 and 1808: 91 us, 5056 and 4944: 71; with an odd number they cost 2048 x 50001 bf16 16 %)
   a.part = a.chunks % 2 ? part * 8 : ((a.units + a.chunks - 1) / a.chunks + 7) / 8 * 64;
-  if (rows > kMaxGrid / a.chunks) return ppoxp_fail(PPO_XP_EINVAL, "%s: %zu rows of %zu are too many for one launch", who, rows, vocab);
+  const size_t blocks = a.rows_per > 1 ? rows / a.rows_per + (rows % a.rows_per != 0) : rows * a.chunks;
+  if (rows > kMaxRows || !one_launch(blocks, 256)) return ppoxp_fail(PPO_XP_EINVAL, "%s: %zu rows of %zu are too many for one launch", who, rows, vocab);
   a.magic = ((1u << 20) + a.units - 1) / a.units;
   a.scan_log2 = 8;
   while (a.scan_log2 && (256u >> a.scan_log2) < a.rows_per) --a.scan_log2;
   a.r = *rules;
   DeviceGuard dev(device, who);
   if (dev.rc()) return dev.rc();
-  const dim3 grid((unsigned)(a.rows_per > 1 ? (rows + a.rows_per - 1) / a.rows_per : rows * a.chunks));
+  const dim3 grid((unsigned)blocks);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == PPO_XP_F32) launch_shape<float>(a, grid, narrow, s, hist, backward);
   else if (dtype == PPO_XP_BF16) launch_shape<__bf16>(a, grid, narrow, s, hist, backward);
@@ -1152,34 +1153,49 @@ void launch_stats(const Plan &p, const PolicyArgs &a, Softmax *parts, float *pic
 // `kWaves`: waves a CU holds of the kernel with that many vectors (its registers: 22 and 4 a vector, 8 of floats).
 constexpr int row_waves(int regs) { return 512 / ((regs + 7) / 8 * 8) >= 8 ? 32 : 512 / ((regs + 7) / 8 * 8) * 4; }
 
+struct RowChoice { int registers; unsigned threads; };    // 16-byte registers of a thread's vectors; 0: the row is too long for them
+
+template <typename T>
+RowChoice row_choice(const PolicyArgs &a) {
+  constexpr int kScale = sizeof(T) / 2;                 // 16-byte registers of 8 elements
+  static const int choices[] = {4, 6, 8, 10, 12, 14, 16};
+  const bool odd = (uintptr_t)a.logits % 4 || (a.rows > 1 && a.stride * sizeof(T) % 4);   // some row starts with half a word
+  const unsigned vecs = (a.vocab + odd + 7) / 8;
+  RowChoice best{0, 1024};
+  int rows = 0;
+  for (int c : choices) {
+    const unsigned waves = (vecs + c / kScale * 64 - 1) / (c / kScale * 64);
+    const int held = waves <= 16 ? row_waves(22 + 4 * c) / (int)waves : 0;
+    if (held > rows) { rows = held; best = RowChoice{c, waves * 64}; }
+  }
+  return best;
+}
+
 template <typename T, int NV>
-void launch_row_as(const PolicyArgs &a, unsigned vecs, hipStream_t s) {
-  const unsigned threads = ((vecs + NV - 1) / NV + 63) / 64 * 64;
+void launch_row_as(const PolicyArgs &a, unsigned threads, hipStream_t s) {
   hipLaunchKernelGGL((policy_loss_row_kernel<T, NV>), dim3((unsigned)a.rows), dim3(threads), 0, s, a);
 }
 
 template <typename T>
 void launch_row(const PolicyArgs &a, hipStream_t s) {
-  constexpr int kScale = sizeof(T) / 2;                 // 16-byte registers of 8 elements
-  static const int choices[] = {4, 6, 8, 10, 12, 14, 16};
-  const bool odd = (uintptr_t)a.logits % 4 || (a.rows > 1 && a.stride * sizeof(T) % 4);   // some row starts with half a word
-  const unsigned vecs = (a.vocab + odd + 7) / 8;
-  int best = 0, rows = 0;
-  for (int c : choices) {
-    const unsigned waves = (vecs + c / kScale * 64 - 1) / (c / kScale * 64);
-    const int held = waves <= 16 ? row_waves(22 + 4 * c) / (int)waves : 0;
-    if (held > rows) { rows = held; best = c; }
+  constexpr int kScale = sizeof(T) / 2;
+  const RowChoice r = row_choice<T>(a);
+  switch (r.registers) {
+    case 4: launch_row_as<T, 4 / kScale>(a, r.threads, s); break;
+    case 6: launch_row_as<T, 6 / kScale>(a, r.threads, s); break;
+    case 8: launch_row_as<T, 8 / kScale>(a, r.threads, s); break;
+    case 10: launch_row_as<T, 10 / kScale>(a, r.threads, s); break;
+    case 12: launch_row_as<T, 12 / kScale>(a, r.threads, s); break;
+    case 14: launch_row_as<T, 14 / kScale>(a, r.threads, s); break;
+    case 16: launch_row_as<T, 16 / kScale>(a, r.threads, s); break;
+    default: hipLaunchKernelGGL(policy_loss_long_kernel<T>, dim3((unsigned)a.rows), dim3(r.threads), 0, s, a); break;
   }
-  switch (best) {
-    case 4: launch_row_as<T, 4 / kScale>(a, vecs, s); break;
-    case 6: launch_row_as<T, 6 / kScale>(a, vecs, s); break;
-    case 8: launch_row_as<T, 8 / kScale>(a, vecs, s); break;
-    case 10: launch_row_as<T, 10 / kScale>(a, vecs, s); break;
-    case 12: launch_row_as<T, 12 / kScale>(a, vecs, s); break;
-    case 14: launch_row_as<T, 14 / kScale>(a, vecs, s); break;
-    case 16: launch_row_as<T, 16 / kScale>(a, vecs, s); break;
-    default: hipLaunchKernelGGL(policy_loss_long_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, s, a); break;
-  }
+}
+
+// Whether the call's largest launch can be dispatched; `threads`: of a row's workgroup where it has one.
+bool fits(const Plan &p, size_t rows, unsigned threads) {
+  if (rows > kMaxRows) return false;
+  return p.blocks || (p.route == kSplit ? one_launch(rows * p.chunks, 256) : one_launch(rows, threads));
 }
 
 template <typename T>
@@ -1231,8 +1247,9 @@ int ppo_xp_action_stats(int device, void *stream, int dtype, const void *logits,
   if (int rc = check_rows("action_stats", dtype, logits, logits_stride, rows, vocab)) return rc;
   if (rows == 0 || vocab == 0) return 0;
   if (!actions || !neglogps || !entropies) return ppoxp_fail(PPO_XP_EINVAL, "action_stats: NULL argument");
-  if (rows > kMaxGrid) return ppoxp_fail(PPO_XP_EINVAL, "action_stats: %zu rows are too many for one launch", rows);
   const Plan p = plan_of(rows, vocab, false, dtype == PPO_XP_F32);
+  if (!fits(p, rows, 256))                                   // 1024 threads a row only below 256 rows
+    return ppoxp_fail(PPO_XP_EINVAL, "action_stats: %zu rows of %zu are too many for one launch", rows, vocab);
   if (int rc = check_workspace("action_stats", p, workspace, workspace_bytes)) return rc;
   PolicyArgs a{};
   a.logits = logits; a.stride = logits_stride; a.actions = actions; a.neglogps = neglogps; a.entropies = entropies;
@@ -1262,15 +1279,16 @@ int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, 
   if (!b || !b->actions || !b->old_values || !b->old_neglogps || !b->returns || !b->advantages || !b->values || !dvalues || !neglogps ||
       !entropies || !stats)
     return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: NULL argument");
-  if (rows > kMaxGrid) return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: %zu rows are too many for one launch", rows);
   const Plan p = plan_of(rows, vocab, true, dtype == PPO_XP_F32);
-  if (int rc = check_workspace("policy_loss", p, workspace, workspace_bytes)) return rc;
   PolicyArgs a{};
   a.logits = logits; a.stride = logits_stride; a.actions = b->actions; a.neglogps = neglogps; a.entropies = entropies;
   a.vocab = (unsigned)vocab; a.rows = rows;
   a.old_values = b->old_values; a.old_neglogps = b->old_neglogps; a.returns = b->returns; a.advantages = b->advantages; a.values = b->values;
   a.clip = clip; a.ent_coef = ent_coef; a.vf_coef = vf_coef; a.inv_denom = (float)(1. / denom);
   a.dlogits = dlogits; a.dstride = dlogits_stride; a.dvalues = dvalues; a.partials = (double *)workspace;
+  if (!fits(p, rows, (dtype == PPO_XP_F32 ? row_choice<float>(a) : row_choice<__bf16>(a)).threads))    // of the type, its size matters
+    return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: %zu rows of %zu are too many for one launch", rows, vocab);
+  if (int rc = check_workspace("policy_loss", p, workspace, workspace_bytes)) return rc;
   DeviceGuard dev(device, "policy_loss");
   if (dev.rc()) return dev.rc();
   char *ws = (char *)workspace;

@@ -263,29 +263,34 @@ int check_store(const char *who, int dtype, size_t width, int format, size_t gro
 // Several units a lane hide the latency of large calls (a small one would not reach every CU): two where rows are read whole (32768 x
 // 4096 bf16: 70 us, with four 88, with one 83), four where they are gathered.
 constexpr size_t kManyUnits = size_t(256) * 256 * 4;
+constexpr int kWriteUnits = 2, kReadUnits = 4;
+size_t blocks_of(size_t total, int units) {      // `units` a lane, where there are many
+  const size_t per = 256 * (total >= kManyUnits ? units : 1);
+  return total / per + (total % per != 0);
+}
 
 template <typename T, int U>
 void launch_quant(int format, hipStream_t s, const QuantArgs &a) {
-  const dim3 grid((unsigned)((a.total + 256 * U - 1) / (256 * U)));
+  const dim3 grid((unsigned)blocks_of(a.total, kWriteUnits));
   if (format == PPO_XP_Q_INT8) hipLaunchKernelGGL((quantize_rows_kernel<T, PPO_XP_Q_INT8, U>), grid, dim3(256), 0, s, a);
   else if (format == PPO_XP_Q_E4M3) hipLaunchKernelGGL((quantize_rows_kernel<T, PPO_XP_Q_E4M3, U>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((quantize_rows_kernel<T, PPO_XP_Q_INT4, U>), grid, dim3(256), 0, s, a);
 }
 template <typename T>
 void launch_quant(int format, hipStream_t s, const QuantArgs &a) {
-  if (a.total >= kManyUnits) launch_quant<T, 2>(format, s, a);
+  if (a.total >= kManyUnits) launch_quant<T, kWriteUnits>(format, s, a);
   else launch_quant<T, 1>(format, s, a);
 }
 template <typename T, int U>
 void launch_dequant(int format, hipStream_t s, const DequantArgs &a) {
-  const dim3 grid((unsigned)((a.total + 256 * U - 1) / (256 * U)));
+  const dim3 grid((unsigned)blocks_of(a.total, kReadUnits));
   if (format == PPO_XP_Q_INT8) hipLaunchKernelGGL((dequantize_rows_kernel<T, PPO_XP_Q_INT8, U>), grid, dim3(256), 0, s, a);
   else if (format == PPO_XP_Q_E4M3) hipLaunchKernelGGL((dequantize_rows_kernel<T, PPO_XP_Q_E4M3, U>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((dequantize_rows_kernel<T, PPO_XP_Q_INT4, U>), grid, dim3(256), 0, s, a);
 }
 template <typename T>
 void launch_dequant(int format, hipStream_t s, const DequantArgs &a) {
-  if (a.total >= kManyUnits) launch_dequant<T, 4>(format, s, a);
+  if (a.total >= kManyUnits) launch_dequant<T, kReadUnits>(format, s, a);
   else launch_dequant<T, 1>(format, s, a);
 }
 
@@ -307,7 +312,7 @@ int ppo_xp_quantize_rows(int device, void *stream, int dtype, const void *rows, 
   a.rows_stride = rows_stride; a.codes_stride = codes_stride; a.scales_stride = scales_stride;
   a.width = (unsigned)width; a.at = at; a.lanes_log2 = (unsigned)log2_of_group(group) - 3;
   a.slots = (unsigned)(((width + group - 1) / group) * (group / 8));
-  if (n > (~size_t(0)) / a.slots || (n * a.slots + 255) / 256 > kMaxGrid)
+  if (n > (~size_t(0)) / a.slots || !one_launch(blocks_of(n * a.slots, kWriteUnits), 256))
     return ppoxp_fail(PPO_XP_EINVAL, "quantize_rows: %zu rows of %zu are too many for one launch", n, width);
   a.total = n * a.slots;
   DeviceGuard dev(device, "quantize_rows");
@@ -337,7 +342,7 @@ int ppo_xp_dequantize_rows(int device, void *stream, int dtype, const void *code
   a.group_log2 = (unsigned)log2_of_group(group);
   const size_t E = 16 / dtype_bytes(dtype);
   a.slots = (unsigned)((width + E - 1) / E);
-  if (n > (~size_t(0)) / a.slots || (n * a.slots + 255) / 256 > kMaxGrid)
+  if (n > (~size_t(0)) / a.slots || !one_launch(blocks_of(n * a.slots, kReadUnits), 256))
     return ppoxp_fail(PPO_XP_EINVAL, "dequantize_rows: %zu rows of %zu are too many for one launch", n, width);
   a.total = n * a.slots;
   DeviceGuard dev(device, "dequantize_rows");
