@@ -402,7 +402,7 @@ typedef struct ppo_xp_policy_batch {
  *   loss = (sum pg + vf_coef sum vl - ent_coef sum H) / denom
  * stats[6] = loss, policy, value, entropy, sum (nlp - old)^2 / 2, rows with |ratio - 1| > clip - each over denom.  dlogits
  * (the logits' type; may be the logits themselves), dvalues [rows]; neglogps and entropies [rows] as ppo_xp_action_stats
- * gives them.  denom > 0: the rows to divide by, padding not counted.  A row that is -inf throughout has gradient 0. */
+ * gives them.  denom >= 2^-127: the rows to divide by, padding not counted.  A row that is -inf throughout has gradient 0. */
 int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, int64_t logits_stride,
                        const ppo_xp_policy_batch *batch, float clip, float ent_coef, float vf_coef, double denom,
                        void *dlogits, int64_t dlogits_stride, float *dvalues, float *neglogps, float *entropies,

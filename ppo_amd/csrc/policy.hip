@@ -1274,7 +1274,8 @@ int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, 
   if (int rc = check_rows("policy_loss", dtype, dlogits, dlogits_stride, rows, vocab)) return rc;
   if (!(clip >= 0.f) || !std::isfinite(clip) || !std::isfinite(ent_coef) || !std::isfinite(vf_coef))
     return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: clip %g (>= 0), ent_coef %g and vf_coef %g must be finite", clip, ent_coef, vf_coef);
-  if (!(denom > 0.) || !std::isfinite(denom)) return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: denom %g must be finite and > 0", denom);
+  if (!(denom > 0.) || !std::isfinite(denom) || !std::isfinite((float)(1. / denom)))     // gradients are scaled by the 32-bit 1 / denom
+    return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: denom %g must be finite and at least 2^-127", denom);
   if (rows == 0 || vocab == 0) return 0;
   if (!b || !b->actions || !b->old_values || !b->old_neglogps || !b->returns || !b->advantages || !b->values || !dvalues || !neglogps ||
       !entropies || !stats)

@@ -40,3 +40,9 @@ def test_more_stored_rows_than_a_dispatch_counts(dtype):
     refused(L.ppo_xp_quantize_rows(0, None, dtype, P, 64, 1 << 30, 64, 1, 64, P, 64, P, 1, 1 << 40, 0), "too many")
     n = (1 << 34) // (16 if dtype == 0 else 8)
     refused(L.ppo_xp_dequantize_rows(0, None, dtype, P, 64, P, 1, 8, 64, 1, 64, P, 32, 0, n, P, 64), "too many")
+
+
+def test_denominators_without_a_finite_reciprocal():
+    batch = struct.pack("6Q", *(P,) * 6)
+    for denom in (2.0 ** -128, 1e-39, 1e-300, 5e-324):
+        refused(L.ppo_xp_policy_loss(0, None, 0, P, 100, batch, 0.2, 0.01, 0.5, denom, P, 100, P, P, P, P, 4, 100, P, 1 << 40), "denom")
