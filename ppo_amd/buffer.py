@@ -115,9 +115,11 @@ class ExperienceBuffer:
         other streams and the pass itself are the ordinary ones; a minibatch's rows are read when the iterator yields it: insert again
         only after that (as with streaming passes).  Inserts and reads may run on different torch streams."""
         import torch
-        from .quant import QuantizedRows
+        from .quant import QuantizedRows, _check
+        dtype = torch.float32 if dtype is None else dtype
+        _check(row_size, format, group, dtype)
         self = cls(num_envs, 1, capacity, gamma, lam, device)      # the handle's own rows: one unused float
-        self.rows_dtype = torch.float32 if dtype is None else dtype
+        self.rows_dtype = dtype
         self.rows = self._on_rows(lambda: QuantizedRows(self.capacity * self.num_envs, row_size, format, group, device))
         self._no_obs = self._on_rows(lambda: torch.zeros(self.num_envs, 1, device=self.rows.codes.device))
         return self

@@ -11,6 +11,7 @@ from ._lib import EINVAL, PpoXpPanic
 
 _call = _lib.torchcall()                          # csrc/torchcall.cpp
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_GROUPS = (16, 32, 64, 128, 256, 512)
 
 #: format -> (PPO_XP_Q_*, type of the codes)
 FORMATS = {"int8": (1, torch.int8), "e4m3": (2, torch.float8_e4m3fn), "int4": (3, torch.uint8)}
@@ -18,6 +19,18 @@ FORMATS = {"int8": (1, torch.int8), "e4m3": (2, torch.float8_e4m3fn), "int4": (3
 
 def _panic(msg):
     raise PpoXpPanic(EINVAL, msg)
+
+
+def _check(row_size, format, group, dtype=torch.float32):
+    """What a store is made of, and the type its rows are read as."""
+    if format not in FORMATS:
+        _panic(f"QuantizedRows: format {format!r} is none of {sorted(FORMATS)}")
+    if not 1 <= row_size <= 1 << 24:
+        _panic(f"QuantizedRows: rows of {row_size} elements (1 .. 2^24 expected)")
+    if group not in _GROUPS:
+        _panic(f"QuantizedRows: group {group} is none of {list(_GROUPS)}")
+    if dtype not in _DTYPES:
+        _panic(f"QuantizedRows: rows are read as f32, bf16 or f16, not {dtype}")
 
 
 class QuantizedRows:
@@ -28,10 +41,9 @@ class QuantizedRows:
     Like the buffer's streams the rows start out as zeros.  Calls run on torch's current stream and do not synchronise."""
 
     def __init__(self, num_rows: int, row_size: int, format: str = "int8", group: int = 64, device: int = 0):
-        if format not in FORMATS:
-            _panic(f"QuantizedRows: format {format!r} is none of {sorted(FORMATS)}")
-        if num_rows < 0 or row_size < 1 or group < 1:
-            _panic("QuantizedRows: num_rows >= 0, row_size and group >= 1 expected")
+        _check(row_size, format, group)
+        if num_rows < 0:
+            _panic(f"QuantizedRows: {num_rows} rows")
         dev = torch.device("cuda", int(device))
         nbytes = (row_size + 1) // 2 if format == "int4" else row_size
         codes = torch.zeros(num_rows, nbytes, dtype=torch.uint8, device=dev).view(FORMATS[format][1])
@@ -45,8 +57,7 @@ class QuantizedRows:
         return self
 
     def _init(self, codes, scales, row_size, format, group):
-        if format not in FORMATS:
-            _panic(f"QuantizedRows: format {format!r} is none of {sorted(FORMATS)}")
+        _check(row_size, format, group)
         kind, dtype = FORMATS[format]
         nbytes = (row_size + 1) // 2 if format == "int4" else row_size
         if not codes.is_cuda or codes.dtype is not dtype or codes.dim() != 2 or codes.shape[1] != nbytes or scales.dtype is not torch.float32 \
