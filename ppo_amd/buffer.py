@@ -96,6 +96,7 @@ class ExperienceBuffer:
         self._L = L
         self.streaming = False
         self.rows, self.rows_dtype = None, None   # new_quantized: the store of observation rows
+        self._row = self.obs_size                 # floats of an observation row in the handle's own memory
 
     # -- constructors with the reference's names ------------------------------------------
     @classmethod
@@ -119,7 +120,7 @@ class ExperienceBuffer:
         dtype = torch.float32 if dtype is None else dtype
         _check(row_size, format, group, dtype)
         self = cls(num_envs, 1, capacity, gamma, lam, device)      # the handle's own rows: one unused float
-        self.rows_dtype = dtype
+        self.obs_size, self.rows_dtype = int(row_size), dtype
         self.rows = self._on_rows(lambda: QuantizedRows(self.capacity * self.num_envs, row_size, format, group, device))
         self._no_obs = self._on_rows(lambda: torch.zeros(self.num_envs, 1, device=self.rows.codes.device))
         return self
@@ -188,7 +189,7 @@ class ExperienceBuffer:
         rewards, vals, neglogps = (_np(x, np.float32, n) for x, n in ((rewards, "rewards"), (vals, "vals"), (neglogps, "neglogps")))
         actions = _np(actions, np.uint64, "actions")
         dones = _np(dones, np.uint8, "dones")
-        if obs.ndim != 2 or obs.shape[1] != self.obs_size:
+        if obs.ndim != 2 or obs.shape[1] != self._row:
             raise PpoXpPanic(_lib.EINVAL, f"add_experience: obs must be [n, {self.obs_size}] (obs: &[[f32; OBS_SIZE]], buffer.rs:86)")
         n = obs.shape[0]
         for name, a in (("rewards", rewards), ("actions", actions), ("vals", vals), ("dones", dones), ("neglogps", neglogps)):
@@ -209,7 +210,7 @@ class ExperienceBuffer:
         actions = _np(actions, np.uint64, "actions")
         dones = _np(dones, np.uint8, "dones")
         steps = rewards.shape[0]
-        if obs.shape != (steps, self.num_envs, self.obs_size) or any(
+        if obs.shape != (steps, self.num_envs, self._row) or any(
                 a.shape != (steps, self.num_envs) for a in (rewards, actions, vals, dones, neglogps)):
             raise PpoXpPanic(_lib.EINVAL, "add_many: shape mismatch")
         if self.rows is not None:
@@ -230,7 +231,7 @@ class ExperienceBuffer:
         for t, w in zip(ts, want):
             if not (t.is_cuda and t.is_contiguous() and t.dtype == w):
                 raise PpoXpPanic(_lib.EINVAL, "add_experience_device: contiguous CUDA tensors of f32/f32/i64/f32/f32/f32 expected")
-        if obs.shape != (self.num_envs, self.obs_size) or any(t.shape != (self.num_envs,) for t in ts[1:]):
+        if obs.shape != (self.num_envs, self._row) or any(t.shape != (self.num_envs,) for t in ts[1:]):
             raise PpoXpPanic(_lib.EINVAL, "add_experience_device: length != NUM_ENVS (reference panics, buffer.rs:97-112)")
         # the six copies are only ENQUEUED on the handle's stream: order them after the producers (torch's
         # current stream) and order torch's stream after them, so that neither an in-place update of the

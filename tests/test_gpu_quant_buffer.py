@@ -28,3 +28,18 @@ def test_host_rows_of_another_layout_are_refused():
     want.write(torch.from_numpy(np.concatenate([one[None], many[:2]]).reshape(T * N, D)).cuda())
     assert torch.equal(buf.training_views()[0], want.read())
     buf.close()
+
+
+def test_its_row_size_is_its_obs_size():
+    import ppo_amd
+    buf = ppo_amd.ExperienceBuffer.new_quantized(N, D, T)
+    assert buf.obs_size == D
+    f = np.zeros(N, np.float32)
+    buf.add_experience(np.zeros((N, buf.obs_size), np.float32), f, f.astype(np.uint64), f, f.astype(np.uint8), f)
+    z = torch.zeros(N, device="cuda")
+    buf.add_experience_device(torch.zeros(N, buf.obs_size, device="cuda"), z, z.long(), z, z, z)
+    assert buf.training_views()[0].shape == (2 * N, buf.obs_size)
+    buf.returns(np.zeros(N, np.uint8))
+    for batch in ppo_amd.ExperienceBatcher(buf, 5):
+        assert batch.observations.shape == (5, buf.obs_size)
+    buf.close()
