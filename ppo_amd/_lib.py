@@ -186,6 +186,18 @@ def torchcall():
     return _torchcall
 
 
+class _Bound:
+    """torchcall()'s functions, bound at the first call of each: importing the package needs no more than libppo_xp.so."""
+
+    def __getattr__(self, name):
+        f = getattr(torchcall(), name)
+        setattr(self, name, f)
+        return f
+
+
+bound = _Bound()
+
+
 def last_error() -> str:
     return (load().ppo_xp_last_error() or b"").decode()
 

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 
-_call = _lib.torchcall()                          # csrc/torchcall.cpp: arguments checked, results allocated, launched
+_call = _lib.bound                                # csrc/torchcall.cpp: arguments checked, results allocated, launched
 
 
 def shape_logits(logits, *, history=None, hist_row=None, hist_begin=None, gen_begin=None, hist_end=None, repetition=1.0, presence=0.0,

@@ -9,7 +9,7 @@ import torch
 from . import _lib
 from ._lib import EINVAL, PpoXpPanic
 
-_call = _lib.torchcall()                          # csrc/torchcall.cpp
+_call = _lib.bound                                # csrc/torchcall.cpp
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _GROUPS = (16, 32, 64, 128, 256, 512)
 
