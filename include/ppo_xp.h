@@ -420,7 +420,7 @@ enum { PPO_XP_Q_INT8 = 1, PPO_XP_Q_E4M3 = 2, PPO_XP_Q_INT4 = 3 };
 int ppo_xp_quantize_rows(int device, void *stream, int dtype, const void *rows, int64_t rows_stride, size_t n,
                          size_t width, int format, size_t group, void *codes, int64_t codes_stride, float *scales,
                          int64_t scales_stride, size_t store_rows, size_t at);
-/* out[j] = store row index[j], as dtype (code * scale, one rounding).  index: index_bits 32 (unsigned) or 64 wide, an entry
+/* out[j] = store row index[j]: code * scale in 32 bits, rounded to dtype.  index: index_bits 32 (unsigned) or 64 wide, an entry
  * outside 0..store_rows reads the last row (as in a pass, a bad index never faults); NULL: rows at .. at + n.  */
 int ppo_xp_dequantize_rows(int device, void *stream, int dtype, const void *codes, int64_t codes_stride,
                            const float *scales, int64_t scales_stride, size_t store_rows, size_t width, int format,

@@ -75,3 +75,20 @@ def test_rows_written_in_place_are_seen_by_autograd():
         assert torch.equal(store.read(index, out=out), store.read(index))
         s = ppo_amd.QuantizedRows(8, 64, "int8", 32)
         s.write(torch.ones(8, 64, device="cuda"))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3", "int4"])
+@pytest.mark.parametrize("n", [2000, 40000])
+def test_16_bit_reads_are_the_32_bit_read_rounded(n, fmt):
+    """The product of a code and a scale has up to 31 significant bits: it is rounded to 32-bit numbers, and those to 16 bits, at every
+    place of a row alike.  Among this many products some lie next to a border between two 16-bit numbers."""
+    import ppo_amd
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n)
+    for width in (75, 64, 8):
+        x = torch.randn(n, width, generator=g, device="cuda") * torch.rand(width, generator=g, device="cuda").pow(-0.5)
+        store = ppo_amd.QuantizedRows(n, width, fmt, 16)
+        for k in range(max(1, 200000 // n)):
+            store.write(x * (1.0 + k / 64.0))
+            for dtype in (torch.float16, torch.bfloat16):
+                assert torch.equal(store.read(dtype=dtype), store.read().to(dtype))
