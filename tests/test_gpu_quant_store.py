@@ -92,3 +92,105 @@ def test_16_bit_reads_are_the_32_bit_read_rounded(n, fmt):
             store.write(x * (1.0 + k / 64.0))
             for dtype in (torch.float16, torch.bfloat16):
                 assert torch.equal(store.read(dtype=dtype), store.read().to(dtype))
+
+
+# ---- calls large enough for several units a lane ------------------------------------------------------------------------------
+
+MANY_UNITS = 256 * 256 * 4          # from here on a lane writes two units of 8 elements and reads four of 16 bytes
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3", "int4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,width,group", [(40000, 75, 32), (270001, 8, 16), (66001, 31, 16), (520, 4100, 32), (33000, 64, 64), (8193, 257, 256), (131073, 2, 16)])
+def test_large_calls(n, width, group, dtype, fmt):
+    """Ragged and even widths, apart and together, with a last workgroup that is partly filled: written, and read in order, by
+    indexes of both widths and by bad ones."""
+    import ppo_amd
+    from test_gpu_quant_rows import code_values, quantized64, read64
+    units = n * (-(-width // group) * (group // 8))
+    assert units >= MANY_UNITS
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n + width)
+    wide = (torch.randn(n, width + 3, generator=g, device="cuda") * torch.rand(width + 3, generator=g, device="cuda").pow(-0.5)).to(dtype)
+    wide[n // 3] = 0
+    wide[n // 2, 1] = float("nan")
+    q, s = quantized64(wide[:, 1:width + 1], fmt, group)
+    bytes_ = (width + 1) // 2 if fmt == "int4" else width
+    plain = ppo_amd.QuantizedRows(n, width, fmt, group)
+    plain.write(wide[:, 1:width + 1])
+    # the same rows, contiguous, into a store whose rows lie apart, behind rows of others
+    kind = plain.codes.dtype
+    codes, scales = torch.full((n + 5, bytes_ + 3), 9, dtype=torch.uint8, device="cuda"), torch.full((n + 5, s.shape[1] + 2), 5.0, device="cuda")
+    apart = ppo_amd.QuantizedRows.of(codes.view(kind)[:, 1:bytes_ + 1], scales[:, 1:-1], width, fmt, group)
+    apart.write(wide[:, 1:width + 1].contiguous(), 2)
+    same = lambda x, y: torch.equal(x.nan_to_num(-7e30), y.nan_to_num(-7e30))  # noqa: E731
+    assert same(plain.scales.double(), s) and torch.equal(code_values(plain), q)
+    assert torch.equal(codes[2:n + 2, 1:bytes_ + 1], plain.codes.view(torch.uint8)) and same(scales[2:n + 2, 1:-1], plain.scales)
+    assert torch.all(codes[:2] == 9) and torch.all(codes[n + 2:] == 9) and torch.all(codes[:, 0] == 9) and torch.all(codes[:, bytes_ + 1:] == 9)
+    assert torch.all(scales[:2] == 5) and torch.all(scales[n + 2:] == 5) and torch.all(scales[:, 0] == 5) and torch.all(scales[:, -1] == 5)
+    index = torch.randint(0, n, (n + 77,), generator=g, device="cuda")
+    index[5], index[-1], index[-2] = -1, n + 2 ** 31 - 1 - n, n
+    rows = index.clone()
+    rows[(index < 0) | (index >= n)] = n - 1
+    for out_t in (torch.float32, torch.bfloat16, torch.float16):
+        want = read64(q, s, group, out_t)
+        assert same(plain.read(dtype=out_t), want)
+        out = torch.full((n, width + 5), 3.0, dtype=out_t, device="cuda")
+        assert same(apart.read(slice(2, n + 2), dtype=out_t, out=out[:, 3:width + 3]), want)
+        assert torch.all(out[:, :3] == 3) and torch.all(out[:, width + 3:] == 3)
+        want = want[rows]
+        assert same(plain.read(index, dtype=out_t), want) and same(plain.read(index.int(), dtype=out_t), want)
+
+
+@pytest.fixture
+def empty_cache():
+    torch.cuda.empty_cache()
+    yield
+    torch.cuda.empty_cache()
+
+
+def room(gib):
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GiB")
+
+
+def test_reads_of_more_than_2_32_units(empty_cache):
+    """Units are numbered in 64 bits from there on: 69 GB of output."""
+    import ppo_amd
+    room(80)
+    store = ppo_amd.QuantizedRows(5, 64, "int8", 64)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    store.write(torch.randn(5, 64, generator=g, device="cuda"))
+    each = store.read()
+    n = (1 << 28) + 5                                          # 16 units a row
+    index = torch.zeros(n, dtype=torch.int32, device="cuda")
+    for at in (0, 1 << 14, (1 << 28) - 2, n - 5):              # the first rows, those round the 2^32nd unit, the last ones
+        index[at:at + 5] = torch.tensor([1, 2, 3, 4, 2], dtype=torch.int32, device="cuda")
+    out = store.read(index)
+    for lo in range(0, n, 1 << 24):
+        assert torch.equal(out[lo:lo + (1 << 24)], each[index[lo:lo + (1 << 24)].long()])
+
+
+def test_writes_of_more_than_2_32_units(empty_cache):
+    import ppo_amd
+    room(110)
+    n = (1 << 29) + 5                                          # 8 units a row, 69 GB of input
+    x = torch.zeros(n, 64, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    places = (0, 1 << 14, (1 << 29) - 2, n - 5)
+    for at in places:
+        x[at:at + 5] = torch.randn(5, 64, generator=g, device="cuda").to(torch.bfloat16)
+    store = ppo_amd.QuantizedRows(n, 64, "int4", 64)
+    store.codes.fill_(0xff)
+    store.write(x)
+    left = torch.ones(n, dtype=torch.bool, device="cuda")
+    for at in places:
+        few = ppo_amd.QuantizedRows(5, 64, "int4", 64)
+        few.write(x[at:at + 5])
+        assert torch.equal(store.codes[at:at + 5], few.codes) and torch.equal(store.scales[at:at + 5], few.scales)
+        left[at:at + 5] = False
+    for lo in range(0, n, 1 << 26):
+        here = left[lo:lo + (1 << 26)]
+        assert not (store.codes[lo:lo + (1 << 26)].view(torch.int64).ne(0).any(1) & here).any() and not (store.scales[lo:lo + (1 << 26), 0].ne(0) & here).any()
