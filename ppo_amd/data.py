@@ -132,6 +132,10 @@ class ExperienceBatcherIterator:
             if hs is not None:
                 cur.wait_stream(hs)
             buf._pass_perm = None
+        if buf.rows is not None:
+            # reads of quantised rows may still be using the previous pass's permutation
+            cur, hs = buf._order_streams()
+            (cur if hs is None else hs).wait_event(buf._rows_done)
         if perm is not None and hasattr(perm, "is_cuda") and perm.is_cuda:
             import torch
             if perm.numel() != len(batcher) or perm.dtype not in (torch.int32,) or not perm.is_contiguous():
@@ -206,9 +210,12 @@ class ExperienceBatcherIterator:
         ptr = L.ppo_xp_pass_perm_device(buf.handle)      # a keyed bijection is written out on the handle's stream the first time
         if not ptr:
             check(_lib.ESTATE)
+        cur, hs = buf._order_streams()
+        if hs is not None:
+            cur.wait_stream(hs)
         start = min(k * B, M - B)
         index = device_tensor(ptr, (M,), torch.uint32, buf.device, buf)[start:start + B]
-        return buf._on_rows(lambda: buf.rows.read(index, dtype=buf.rows_dtype))      # ... and the next pass's behind this read of it
+        return buf._on_rows(lambda: buf.rows.read(index, dtype=buf.rows_dtype))
 
     def next_host(self, out: "HostBatch | None" = None) -> "HostBatch | None":
         """Iterator::next as the reference's caller sees it (data.rs:166-182 feeds six host Vecs to

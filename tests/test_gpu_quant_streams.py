@@ -166,3 +166,46 @@ def test_a_new_buffer_is_empty_before_anything_is_inserted():
     torch.cuda.synchronize()
     assert torch.equal(got, want) and torch.equal(buf.training_views()[0], want)
     buf.close()
+
+
+def test_a_new_pass_waits_for_reads_by_the_last_permutation():
+    """A pass's permutation is overwritten by the next one only behind the reads that use it, on whichever stream they are."""
+    buf, rows, acts, rest = make(13)
+    want = stored(rows)
+    insert(buf, "device", rows, acts, rest)
+    buf.returns(np.zeros(N, np.uint8))
+    for kw in (dict(bijection=True), dict(device_shuffle=True), {}):
+        for seed in (1, 2):                                         # whatever is allocated once is there
+            for _ in minibatches(buf, T * N, seed=seed, **kw)[0]:
+                pass
+        torch.cuda.synchronize()
+        a, b = torch.cuda.Stream(), torch.cuda.Stream()
+        with torch.cuda.stream(b):
+            it, perm = minibatches(buf, T * N, seed=3, **kw)
+            buf.sync()
+            torch.cuda._sleep(SPIN)
+            got = next(it).observations
+        with torch.cuda.stream(a):
+            second, perm2 = minibatches(buf, T * N, seed=4, **kw)
+            got2 = next(second).observations
+        torch.cuda.synchronize()
+        assert torch.equal(got, want[torch.from_numpy(perm).cuda()]) and torch.equal(got2, want[torch.from_numpy(perm2).cuda()])
+    buf.close()
+
+
+def test_sync_and_close_wait_for_rows():
+    import ppo_amd
+    _, rows, acts, rest = make(15)
+    want = stored(rows)
+    buf = ppo_amd.ExperienceBuffer.new_quantized(N, D, T, "int8", 32)
+    a = torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(SPIN)
+        insert(buf, "device", rows, acts, rest)
+    buf.sync()
+    assert torch.equal(buf.rows.read(), want)              # on the default stream, which nothing else orders
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(SPIN)
+        got = buf.stream_view("observations")
+    buf.close()
+    assert torch.equal(got, want)
