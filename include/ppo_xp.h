@@ -400,9 +400,13 @@ typedef struct ppo_xp_policy_batch {
  * new value and ratio = exp(old_neglogp - nlp):
  *   pg = max(-A ratio, -A clamp(ratio, 1 - clip, 1 + clip)),   vl = max((v - ret)^2, (v0 + clamp(v - v0, -clip, clip) - ret)^2) / 2
  *   loss = (sum pg + vf_coef sum vl - ent_coef sum H) / denom
- * stats[6] = loss, policy, value, entropy, sum (nlp - old)^2 / 2, rows with |ratio - 1| > clip - each over denom.  dlogits
- * (the logits' type; may be the logits themselves), dvalues [rows]; neglogps and entropies [rows] as ppo_xp_action_stats
- * gives them.  denom >= 2^-127: the rows to divide by, padding not counted.  A row that is -inf throughout has gradient 0. */
+ * stats[6] = loss, policy, value, entropy, sum (nlp - old)^2 / 2, rows with |ratio - 1| > clip (a NaN is not) - each over denom.
+ * dlogits (the logits' type; may be the logits themselves), dvalues [rows]; neglogps and entropies [rows] as ppo_xp_action_stats
+ * gives them.  A row that is -inf throughout has gradient 0 and its terms by the formula: with a stored neglogp of +inf they are
+ * NaN, so mark rows in which nothing could be drawn as padding.
+ * denom >= 2^-127: the rows to divide by, padding not counted.  stats, dlogits and dvalues are over it alike: rows / S makes them S
+ * times as large, for a power of two exactly.  f16 gradients need that: an element below 2^-25 is rounded to 0, and p g / n is
+ * smaller at some thousand rows of some ten thousand tokens. */
 int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, int64_t logits_stride,
                        const ppo_xp_policy_batch *batch, float clip, float ent_coef, float vf_coef, double denom,
                        void *dlogits, int64_t dlogits_stride, float *dvalues, float *neglogps, float *entropies,

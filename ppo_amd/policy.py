@@ -59,5 +59,6 @@ def policy_loss(logits, values, batch, *, clip=0.2, ent_coef=0.01, vf_coef=0.5, 
 
     logits [rows, vocab] and values f32 [rows]: the policy and critic now; `batch` an ExperienceBatch or anything with its actions,
     values, neglogps, returns and advantages.  Rows whose action is -1 are padding: pass the number of real rows as `denom`
-    (default: all rows).  `out`: where dlogits go, may be `logits` itself."""
+    (default: all rows); rows / S for gradients and statistics S times as large, which f16 gradients need (elements below 2^-25 become
+    0).  `out`: where dlogits go, may be `logits` itself."""
     return PolicyLoss(*_call.loss(logits, values, batch, clip, ent_coef, vf_coef, denom, out))

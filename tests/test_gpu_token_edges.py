@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_policy_ops import BF16, F16, F32, check_shape, gen, half, randn, rules64
+from test_gpu_policy_ops import BF16, F16, F32, batch_of, check_shape, gen, half, policy_inputs, randn, rules64
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -90,3 +90,34 @@ def test_an_infinite_penalty_forbids_the_tokens_it_applies_to(R, V, L, dtype):
         out = ppo_amd.shape_logits(x, history=hist, gen_begin=half_way, **kw)
         forbidden = counted & (inf > 0)[:, None]
         assert torch.all(out[forbidden] == -float("inf")) and torch.equal(out[~forbidden], x[~forbidden])
+
+
+@pytest.mark.parametrize("R,V", [(200, 18), (70, 151), (40, 5000), (6, 70001), (300, 20011)])
+def test_the_denominator_scales_what_is_over_it(R, V):
+    """rows / S with a power of two: statistics and gradients are S times as large to the last bit."""
+    import ppo_amd
+    g, x, a = policy_inputs(R, V, F32, R + V)
+    b = batch_of(g, x, a)
+    S = 2.0 ** 16
+    r, q = (ppo_amd.policy_loss(x, b.new_values, b, denom=n) for n in (float(R), R / S))
+    assert torch.equal(q.stats, r.stats * S) and torch.equal(q.dvalues, r.dvalues * S)
+    assert torch.equal(q.neglogps, r.neglogps) and torch.equal(q.entropies, r.entropies)
+    normal = r.dlogits.abs() >= 2.0 ** -100                    # a factor below 2^-126 has fewer bits, and its product with S keeps them
+    assert torch.equal(q.dlogits[normal], r.dlogits[normal] * S) and torch.all(q.dlogits[~normal].abs() <= 2.0 ** -83)
+
+
+def test_f16_gradients_that_only_a_scale_keeps():
+    import ppo_amd
+    R, V, S = 2048, 30011, 2.0 ** 16
+    g, x, a = policy_inputs(R, V, F16, 5)
+    b = batch_of(g, x, a)
+    want = ppo_amd.policy_loss(x.float(), b.new_values, b).dlogits
+    plain = ppo_amd.policy_loss(x, b.new_values, b).dlogits
+    assert (plain == 0).float().mean() > 0.5                   # what the documentation warns of
+    got = ppo_amd.policy_loss(x, b.new_values, b, denom=R / S).dlogits.float() / S
+    # the same statistics in 32 bits by another route (V / 1000 and 48 additions, as many powers of 2 u, 25 |d| u at most), one rounding to
+    # f16, half of its least subnormal over S
+    size = want.abs() * (half(F16) + 400 * U) + 2.0 ** -25 / S
+    p = torch.softmax(x.float(), 1)
+    ent = 0.01 * p * 40 * 400 * U / R                          # where ln p + H cancels: both below 20 here
+    assert torch.all((got - want).abs() <= size + ent)
