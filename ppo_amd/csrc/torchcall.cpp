@@ -1,6 +1,6 @@
 // _torchcall: the step from torch tensors to the C ABI (include/ppo_xp.h) for the operators on logits and quantised rows - argument
 // checks, allocation of results with torch, torch's current stream.  Host code only; between calls it holds nothing but what setup()
-// gives it.
+// gives it and the address of torch's allocator.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -222,22 +222,25 @@ PyObject *shape_backward(PyObject *const *a) {              // grad, logits, rul
 }
 
 // Results and workspace of one call, each an allocation of torch's of its own on `like`'s device: no result keeps another or the
-// workspace, and calls on two streams and two captured graphs share nothing.  Only the first goes through at::empty, the others ask its
-// allocator directly (at::empty costs the host 0.6 us each: five of them 9.8 us an objective of 64 x 18, this way 8.1).
+// workspace, and calls on two streams and two captured graphs share nothing.  They come straight from the allocator that at::empty
+// takes: five of them cost an objective's host time 0.8 us more than a single at::empty, as five of those 2.3 us.
 class Fresh {
  public:
-  Fresh(const at::Tensor &like, int64_t n)
-      : first(at::empty({n}, at::TensorOptions().dtype(at::kFloat).device(like.device()))), on_(like.device()), from_(first.storage().allocator()) {}
+  explicit Fresh(const at::Tensor &like) : on_(like.device()), from_(allocator(like)) {}
   at::Tensor floats(int64_t n) const {
     at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
-        c10::Storage(c10::Storage::use_byte_size_t(), n * sizeof(float), from_->allocate(n * sizeof(float)), from_, true), first.key_set(), first.dtype());
+        c10::Storage(c10::Storage::use_byte_size_t(), n * sizeof(float), from_->allocate(n * sizeof(float)), from_, true),
+        c10::DispatchKeySet(c10::DispatchKey::CUDA), caffe2::TypeMeta::Make<float>());
     t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
     return t;
   }
   c10::DataPtr memory(size_t bytes) const { return bytes ? from_->allocate(bytes) : c10::DataPtr(); }
-  const at::Tensor first;
 
  private:
+  static c10::Allocator *allocator(const at::Tensor &like) {
+    static c10::Allocator *const a = at::empty({1}, at::TensorOptions().device(like.device())).storage().allocator();
+    return a;
+  }
   const c10::DeviceGuard on_;              // the allocator works on the current device
   c10::Allocator *const from_;
 };
@@ -246,8 +249,8 @@ PyObject *stats(PyObject *const *a) {                       // logits, actions
   const at::Tensor &t = some(a[0], "action_stats");
   const Matrix l = matrix(t, "action_stats");
   const void *actions = vector(a[1], l.rows, at::kLong, l.device, "actions");
-  const Fresh fresh(t, l.rows);
-  const at::Tensor &nlp = fresh.first, ent = fresh.floats(l.rows);
+  const Fresh fresh(t);
+  const at::Tensor nlp = fresh.floats(l.rows), ent = fresh.floats(l.rows);
   if (l.cols == 0) { nlp.zero_(); ent.zero_(); }
   const size_t bytes = g_workspace(l.rows, l.cols, 0);
   const c10::DataPtr ws = fresh.memory(bytes);
@@ -287,8 +290,8 @@ PyObject *loss(PyObject *const *a) {                        // logits, values, b
   }
   Matrix o;
   at::Tensor out = result(a[7], t, who, o);
-  const Fresh fresh(t, l.rows);
-  const at::Tensor &dvalues = fresh.first, nlp = fresh.floats(l.rows), ent = fresh.floats(l.rows), stats = fresh.floats(6);
+  const Fresh fresh(t);
+  const at::Tensor dvalues = fresh.floats(l.rows), nlp = fresh.floats(l.rows), ent = fresh.floats(l.rows), stats = fresh.floats(6);
   if (l.rows == 0 || l.cols == 0)
     for (const at::Tensor *x : {&dvalues, &nlp, &ent, &stats}) x->zero_();
   const size_t bytes = g_workspace(l.rows, l.cols, 1);

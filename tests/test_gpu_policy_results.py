@@ -62,3 +62,23 @@ def test_workspaces_are_given_back():
     before = torch.cuda.memory_allocated()
     kept = [ppo_amd.policy_loss(x, b.new_values, b, out=out).stats for _ in range(100)]
     assert torch.cuda.memory_allocated() - before == 100 * 512 and len(kept) == 100
+
+
+def test_results_come_from_the_pool_that_is_in_use():
+    """Memory of a captured call is the graph's own, and what a kept result holds is freed with it."""
+    import ppo_amd
+    g, x, a = policy_inputs(500, 2100, BF16, 3)
+    b = batch_of(g, x, a)
+    want = ppo_amd.policy_loss(x, b.new_values, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r = ppo_amd.policy_loss(x, b.new_values, b)
+        nlp, ent = ppo_amd.action_stats(x, a)
+    others = [torch.full((500,), 7.0, device="cuda") for _ in range(64)]         # nothing eager lands in the graph's memory
+    for _ in range(3):
+        for t in (r.stats, r.dvalues, r.neglogps, r.entropies, nlp, ent):
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(r.stats, want.stats) and torch.equal(r.neglogps, want.neglogps) and torch.equal(r.dvalues, want.dvalues)
+        assert torch.equal(nlp, ppo_amd.action_stats(x, a)[0]) and all(torch.all(o == 7) for o in others)
