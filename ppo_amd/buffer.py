@@ -286,7 +286,8 @@ class ExperienceBuffer:
 
     def training_views(self):
         """buffer.rs:142-175 → (observations [M, D], actions [M] i64, values [M], neglogps [M]):
-        zero-copy torch views of device memory, storage order (quantised rows: a copy)."""
+        zero-copy torch views of device memory, storage order.  Quantised rows are all read back into a new tensor: a pass over such
+        a buffer needs none of it, ExperienceBatcher(buffer, batch_size) reads each minibatch's rows by themselves."""
         import torch
         v = self._views()
         M, D, d = v.num_steps, self.obs_size, self.device
