@@ -98,7 +98,7 @@ at::Tensor result(PyObject *o, const at::Tensor &like, const char *what, Matrix 
   return out;
 }
 
-// A caller's tensor changes under autograd's eyes: what was saved of it for a backward pass is known to be stale.
+// A caller's tensor has changed under autograd's eyes: what was saved of it for a backward pass is known to be stale.
 void changed(const at::Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -201,8 +201,8 @@ PyObject *shape(PyObject *const *a) {                       // logits, rules, ou
   const ppo_xp_logit_rules r = rules_of(l, a + 1);
   Matrix o;
   at::Tensor out = result(a[1 + RULES], t, "shape_logits", o);
-  written(a[1 + RULES], out);
   done(launch(g_shape, l.device, stream_of(l.device), l.dtype, l.p, l.stride, o.p, o.stride, l.rows, l.cols, &r));
+  written(a[1 + RULES], out);
   return THPVariable_Wrap(out);
 }
 
@@ -216,8 +216,8 @@ PyObject *shape_backward(PyObject *const *a) {              // grad, logits, rul
   const ppo_xp_logit_rules r = rules_of(l, a + 2);
   Matrix o;
   at::Tensor out = result(a[2 + RULES], g, who, o);
-  written(a[2 + RULES], out);
   done(launch(g_shape_backward, l.device, stream_of(l.device), l.dtype, m.p, m.stride, l.p, l.stride, o.p, o.stride, l.rows, l.cols, &r));
+  written(a[2 + RULES], out);
   return THPVariable_Wrap(out);
 }
 
@@ -296,9 +296,9 @@ PyObject *loss(PyObject *const *a) {                        // logits, values, b
     for (const at::Tensor *x : {&dvalues, &nlp, &ent, &stats}) x->zero_();
   const size_t bytes = g_workspace(l.rows, l.cols, 1);
   const c10::DataPtr ws = fresh.memory(bytes);
-  written(a[7], out);
   done(launch(g_loss, l.device, stream_of(l.device), l.dtype, l.p, l.stride, &b, clip, ent_coef, vf, denom, o.p, o.stride, dvalues.data_ptr<float>(),
               nlp.data_ptr<float>(), ent.data_ptr<float>(), stats.data_ptr<float>(), l.rows, l.cols, ws.get(), bytes));
+  written(a[7], out);
   PyObject *r = PyTuple_New(5);
   if (!r) throw Raised{};
   int i = 0;
@@ -342,10 +342,10 @@ PyObject *write(PyObject *const *a) {                       // store, rows, at
   const int64_t at = whole(a[6]);
   if (m.cols != s.width || m.device != s.codes.get_device() || at < 0)
     panic("write: rows of " + num(s.width) + " on cuda:" + num(s.codes.get_device()) + " and at >= 0 expected");
-  changed(s.codes);
-  changed(s.scales);
   done(launch(g_quantize, m.device, stream_of(m.device), m.dtype, m.p, m.stride, m.rows, m.cols, (int)s.kind, s.group, s.codes.data_ptr(), s.codes_stride,
                   s.scales.data_ptr<float>(), s.scales_stride, s.codes.size(0), at));
+  changed(s.codes);
+  changed(s.scales);
   Py_RETURN_NONE;
 }
 
@@ -377,9 +377,9 @@ PyObject *read(PyObject *const *a) {                        // store, index or N
       panic(std::string("read: out must be ") + at::toString(type) + " [" + num(n) + ", " + num(s.width) + "] on the store's device");
   }
   const Matrix o = matrix(out, "read");
-  written(a[9], out);
   done(launch(g_dequantize, device, stream_of(device), (int)dt, s.codes.data_ptr(), s.codes_stride, s.scales.data_ptr<float>(), s.scales_stride, s.codes.size(0),
                     s.width, (int)s.kind, s.group, index, bits, first, n, o.p, o.stride));
+  written(a[9], out);
   return THPVariable_Wrap(out);
 }
 

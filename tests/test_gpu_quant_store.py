@@ -194,3 +194,19 @@ def test_writes_of_more_than_2_32_units(empty_cache):
     for lo in range(0, n, 1 << 26):
         here = left[lo:lo + (1 << 26)]
         assert not (store.codes[lo:lo + (1 << 26)].view(torch.int64).ne(0).any(1) & here).any() and not (store.scales[lo:lo + (1 << 26), 0].ne(0) & here).any()
+
+
+def test_refused_calls_leave_no_trace():
+    """What was saved of a tensor is not stale when the call that would have written it was refused."""
+    import ppo_amd
+    store = ppo_amd.QuantizedRows(8, 64, "int8", 32)
+    out, y = torch.zeros(3, 64, device="cuda"), torch.zeros(4, 10, device="cuda")
+    z, a = torch.zeros(4, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    batch = ppo_amd.ExperienceBatch(None, a, z, z, z, z)
+    for call in (lambda: store.write(torch.zeros(4, 64, device="cuda"), 6), lambda: store.read(slice(4, 8), out=out),
+                 lambda: ppo_amd.shape_logits(y, repetition=-1.0, out=y), lambda: ppo_amd.shape_logits_backward(y, y, temperature=0.0, out=y),
+                 lambda: ppo_amd.policy_loss(y, z, batch, clip=-1.0, out=y)):
+        before = [t._version for t in (store.codes, store.scales, out, y)]
+        with pytest.raises(ppo_amd.PpoXpPanic):
+            call()
+        assert [t._version for t in (store.codes, store.scales, out, y)] == before
