@@ -130,6 +130,8 @@ class ExperienceBuffer:
         """`call`, which writes or reads quantised rows on torch's current stream, behind the last such call, whichever stream that
         ran on.  (Through one event of the buffer's: two torch streams joined with wait_stream make one each time, 9 us of the host's.)"""
         import torch
+        if torch.cuda.is_current_stream_capturing():
+            return call()                         # in a graph: its replays stand where the caller puts them
         cur = torch.cuda.current_stream(self.device)
         cur.wait_event(self._rows_done)
         try:

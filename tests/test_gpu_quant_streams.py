@@ -209,3 +209,22 @@ def test_sync_and_close_wait_for_rows():
         got = buf.stream_view("observations")
     buf.close()
     assert torch.equal(got, want)
+
+
+def test_whole_reads_are_captured():
+    """A read of the rows may be captured: its order with what is outside the graph is the replay's."""
+    buf, rows, acts, rest = make(17)
+    insert(buf, "device", rows, acts, rest)
+    want = buf.stream_view("observations").clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = buf.stream_view("observations") * 2.0
+    for k in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want * 2.0) and torch.equal(buf.stream_view("observations"), want)
+        torch.cuda.synchronize()
+    insert(buf, "device", rows * 3.0, acts, rest)
+    graph.replay()
+    assert torch.equal(out, stored(rows * 3.0) * 2.0)
+    buf.close()
