@@ -238,7 +238,8 @@ class Fresh {
 
  private:
   static c10::Allocator *allocator(const at::Tensor &like) {
-    static c10::Allocator *const a = at::empty({1}, at::TensorOptions().device(like.device())).storage().allocator();
+    static c10::Allocator *a = nullptr;                       // under the interpreter's lock, so no other one is needed
+    if (!a) a = at::empty({1}, at::TensorOptions().device(like.device())).storage().allocator();
     return a;
   }
   const c10::DeviceGuard on_;              // the allocator works on the current device
