@@ -1287,7 +1287,9 @@ int ppo_xp_policy_loss(int device, void *stream, int dtype, const void *logits, 
   a.old_values = b->old_values; a.old_neglogps = b->old_neglogps; a.returns = b->returns; a.advantages = b->advantages; a.values = b->values;
   a.clip = clip; a.ent_coef = ent_coef; a.vf_coef = vf_coef; a.inv_denom = (float)(1. / denom);
   a.dlogits = dlogits; a.dstride = dlogits_stride; a.dvalues = dvalues; a.partials = (double *)workspace;
-  if (!fits(p, rows, (dtype == PPO_XP_F32 ? row_choice<float>(a) : row_choice<__bf16>(a)).threads))    // of the type, its size matters
+  // threads of a row: 1024 at most, which fewer rows fit with; of the type its size matters
+  const unsigned threads = rows >> 22 == 0 ? 1024 : (dtype == PPO_XP_F32 ? row_choice<float>(a) : row_choice<__bf16>(a)).threads;
+  if (!fits(p, rows, threads))
     return ppoxp_fail(PPO_XP_EINVAL, "policy_loss: %zu rows of %zu are too many for one launch", rows, vocab);
   if (int rc = check_workspace("policy_loss", p, workspace, workspace_bytes)) return rc;
   DeviceGuard dev(device, "policy_loss");
