@@ -60,7 +60,7 @@ def minibatches(buf, B, **kw):
 def test_reads_wait_for_inserts_of_another_stream(how, reader):
     buf, rows, acts, rest = make(3)
     want = stored(rows)
-    insert(buf, "device", torch.zeros_like(rows), acts, rest)      # a first round: whatever is allocated once is there
+    insert(buf, "device", torch.zeros_like(rows), acts, rest)      # whatever is allocated once is there
     buf.returns(np.zeros(N, np.uint8))
     for _ in minibatches(buf, T * N, seed=1, bijection=True)[0]:
         pass
@@ -129,7 +129,7 @@ def test_inserts_wait_for_whole_reads(reader):
 
 
 def test_the_same_results_as_on_one_stream():
-    """Collector and learner on streams of their own, several rounds without a host synchronisation between them."""
+    """Collector and learner on streams of their own, several rollouts without a host synchronisation between them."""
     results = []
     for two in (False, True):
         a = torch.cuda.Stream()
